@@ -60,6 +60,8 @@ enum {
  * route in ascending sorted position -- MAGI-2's weighted index_add on bf16
  * tensors (grouped_moe.py:751-756). */
 enum { MIRAI_DTYPE_BF16 = 0, MIRAI_DTYPE_F32 = 1, MIRAI_COMBINE_BF16_ACCUM = 2 };
+/* fp16 matrices (mirai_mxfp4_quantize / _dequantize only) */
+enum { MIRAI_DTYPE_F16 = 3 };
 
 /* Expert weight layouts of the *_ex GEMMs: [G, out, in] (the compressed
  * experts', w1/w3 [E, I, H], w2 [E, H, I]) or [G, in, out] (MAGI-2's W_gate /
@@ -514,6 +516,66 @@ int mirai_moe_down_dh_lora_int8(const void* grad_y, const int32_t* offsets, int3
                                 const void* rank_b, void* dh, mirai_stream_t stream);
 int mirai_swiglu_backward_rotated(const void* dh, const void* gate_up, int64_t rows, int32_t inter, int32_t group,
                                   void* grad_gate_up, mirai_stream_t stream);
+
+/* ------------------------------------------------ MXFP4 (microscaled 4-bit)
+ * Blocks of 32 consecutive elements of a row share the scale 2^e,
+ * e = clamp(floor(log2 max|x|) - 2, -127, 127), stored as the byte e + 127; an
+ * element is x / 2^e rounded to the nearest E2M1 value (0, .5, 1, 1.5, 2, 3, 4, 6
+ * and a sign; ties to the even code, saturating), two codes per byte, the first
+ * element in the low half.  A block with an infinity or a NaN has the byte 255
+ * and reads back as NaN.  (The OCP microscaling format; the reference lists MX
+ * among its storage formats, mirai/core/models/compressed_weights/quantization.)
+ *
+ * Scale bytes are stored in tiles of 128 rows x 4 blocks (512 bytes): row r,
+ * block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b.  An expert key is
+ * packed [E, out, in/2] and scale [E, ceil(out/128), ceil(in/128), 512], zero
+ * bytes past its rows and blocks.  Rows in segments (the routed rows of each
+ * expert) start a new row tile at every segment: their scales are
+ * [tiles, ceil(width/128), 512] with tiles counted segment by segment, in a
+ * buffer of mirai_mxfp4_rows_scale_bytes() bytes (bytes of rows past a
+ * segment's end are not written). */
+typedef struct mirai_mxfp4_weight {
+  const uint8_t* packed; /* {key}_mxfp4       [E, out, in/2]                              */
+  const uint8_t* scale;  /* {key}_mxfp4_scale [E, ceil(out/128), ceil(in/128), 512] tiles */
+} mirai_mxfp4_weight;
+
+size_t mirai_mxfp4_scale_bytes(int32_t num_experts, int64_t out_features, int64_t in_features);
+size_t mirai_mxfp4_rows_scale_bytes(int64_t num_rows, int32_t num_segments, int32_t width);
+
+/* Quantise a [E, out, in] stack (dtype MIRAI_DTYPE_BF16, _F32 or _F16; in % 32 == 0), and
+ * read one back (exact in bf16 and fp32, rounded once to fp16).  Pointers 16-byte aligned. */
+int mirai_mxfp4_quantize(const void* weight, int32_t dtype, int32_t num_experts, int64_t out_features,
+                         int64_t in_features, uint8_t* packed, uint8_t* scale, mirai_stream_t stream);
+int mirai_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scale, int32_t num_experts, int64_t out_features,
+                           int64_t in_features, void* out, int32_t dtype, mirai_stream_t stream);
+
+/* Quantise bf16 activation rows grouped in segments: packed [num_rows, width/2] and the
+ * segment-tiled scales above.  row_index (may be NULL) [num_rows] names the row of x
+ * [x_rows, width] each row is read from (the permute of mirai_permute_rows_bf16 in the same
+ * pass); offsets [num_segments] int32 inclusive row ends, 1..1024 segments.  Rows past the last
+ * segment are not written. */
+int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_index, const int32_t* offsets,
+                              int32_t num_segments, int64_t num_rows, int32_t width, uint8_t* packed, uint8_t* scale,
+                              mirai_stream_t stream);
+
+/* The expert products on MXFP4 operands (tcgen05 block-scaled MMAs, fp32 accumulation):
+ * segment s * num_experts + e holds source s's rows of expert e, offsets ends all
+ * num_sources * num_experts (<= 1024) of them.  hidden and inter are multiples of 32.
+ *
+ * gate/up: h = silu(g) * u, g = x W1^T, u = x W3^T, rounded once to bf16 from fp32.
+ * h [S, I] bf16 and/or its quantised form (h_packed [S, I/2], h_scale: the segment-tiled
+ * scales of width I), of the bf16-rounded h; gate_up (may be NULL) [S, 2I] bf16 is saved for
+ * the backward.  down: y [S, H] = h W2^T; rank_a [S, 64] / rank_b [E*H, 64] bf16 (both or
+ * neither) add a LoRA adapter's rank block, as in mirai_moe_down_lora_bf16.  The backward of
+ * both multiplies the read-back weights (mirai_moe_down_dx_bf16, mirai_moe_gateup_dx_bf16). */
+int mirai_moe_gateup_swiglu_mxfp4(const uint8_t* x_packed, const uint8_t* x_scale, const int32_t* offsets,
+                                  int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
+                                  int32_t inter, const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3, void* h,
+                                  void* gate_up, uint8_t* h_packed, uint8_t* h_scale, mirai_stream_t stream);
+int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const int32_t* offsets, int32_t num_sources,
+                         int32_t num_experts, int64_t num_rows, int32_t inter, int32_t hidden,
+                         const mirai_mxfp4_weight* w2, const void* rank_a, const void* rank_b, void* y,
+                         mirai_stream_t stream);
 
 #ifdef __cplusplus
 }

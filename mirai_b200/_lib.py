@@ -48,6 +48,10 @@ class Int8Weight(ctypes.Structure):
     _fields_ = [("q", c_vp), ("scale", c_vp)]
 
 
+class Mxfp4Weight(ctypes.Structure):
+    _fields_ = [("packed", c_vp), ("scale", c_vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mirai_b200_last_error": (ctypes.c_char_p, []),
@@ -166,6 +170,16 @@ SIGNATURES = {
                                               c_vp, c_vp]),
     "mirai_moe_down_dh_lora_int8": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i64, c_i32, c_i32,
                                                    ctypes.POINTER(Int8Weight), c_vp, c_vp, c_vp, c_vp]),
+    "mirai_mxfp4_scale_bytes": (c_size, [c_i32, c_i64, c_i64]),
+    "mirai_mxfp4_rows_scale_bytes": (c_size, [c_i64, c_i32, c_i32]),
+    "mirai_mxfp4_quantize": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "mirai_mxfp4_dequantize": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i64, c_i64, c_vp, c_i32, c_vp]),
+    "mirai_mxfp4_quantize_rows": (ctypes.c_int, [c_vp, c_i64, c_vp, c_vp, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp]),
+    "mirai_moe_gateup_swiglu_mxfp4": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
+                                                     ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight), c_vp,
+                                                     c_vp, c_vp, c_vp, c_vp]),
+    "mirai_moe_down_mxfp4": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
+                                            ctypes.POINTER(Mxfp4Weight), c_vp, c_vp, c_vp, c_vp]),
 }
 
 _lib = None

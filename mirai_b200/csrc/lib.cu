@@ -8,3 +8,4 @@
 #include "lora.cu"
 #include "exchange.cu"
 #include "rotate.cu"
+#include "mxfp4.cu"

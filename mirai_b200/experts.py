@@ -3,7 +3,7 @@ reference's compressed grouped-expert layer).
 
 ``GroupedExpertWeights`` binds the three expert tensors of one MoE layer
 (gate ``w1`` [E, I, H], up ``w3`` [E, I, H], down ``w2`` [E, H, I], the
-reference's layout, transformer_lingbot_video.py:1143-1145) in one of three
+reference's layout, transformer_lingbot_video.py:1143-1145) in one of four
 storage formats, reading the reference's own buffers in place:
 
 * NF4: ``{key}_nf4``, ``{key}_nf4_absmax``, ``{key}_nf4_nabsmax``,
@@ -12,6 +12,9 @@ storage formats, reading the reference's own buffers in place:
 * INT8: ``{key}_int8`` and ``{key}_scale`` with ``{key}_group_size`` 0
   (plain per-output-channel) or a power of 4 (block-Hadamard rotated,
   quant.py:103-122, 189-260; experts.py:1382-1422);
+* MXFP4: ``{key}_mxfp4`` and ``{key}_mxfp4_scale`` (microscaled 4-bit blocks of
+  32; the forward multiplies the rows in MXFP4 too, the backward passes their
+  gradient straight through the quantiser and multiplies the stored weights);
 * bf16 dense tensors (the LingBot dense grouped experts).
 
 ``B200GroupedExperts`` is an ``nn.Module`` with the reference's construction
@@ -95,6 +98,10 @@ STORAGE: dict[str, tuple[BufferSlot, ...]] = {
         BufferSlot("int8", torch.int8, per_expert=lambda o, i, m: o * i),
         BufferSlot("scale", torch.float32, per_expert=lambda o, i, m: o),
     ),
+    "mxfp4": (
+        BufferSlot("mxfp4", torch.uint8, per_expert=lambda o, i, m: o * i // 2),
+        BufferSlot("mxfp4_scale", torch.uint8, per_expert=lambda o, i, m: -(-o // 128) * -(-i // 128) * 512),
+    ),
 }
 
 
@@ -108,6 +115,8 @@ def storage_problems(fmt: str, key: str, num_experts: int, dense_shape: tuple[in
     _, out_f, in_f = dense_shape
     if fmt == "nf4" and (in_f * out_f) % meta.blocksize:
         problems.append(f"{key}: {out_f}x{in_f} elements are not whole blocks of {meta.blocksize}")
+    if fmt == "mxfp4" and in_f % ops.MXFP4_BLOCK:
+        problems.append(f"{key}: rows of {in_f} are not whole blocks of {ops.MXFP4_BLOCK}")
     for slot in STORAGE[fmt]:
         name = f"{key}_{slot.suffix}"
         t = tensors.get(slot.suffix)
@@ -196,6 +205,19 @@ class GroupedExpertWeights:
             _, inter, hidden = ws["w1"].shape
             return cls("int8", ws["w1"], ws["w3"], ws["w2"], E, hidden, inter,
                        rot_in=groups["w1"], rot_mid=groups["w2"])
+        if fmt == "mxfp4":
+            ws = {}
+            for key in KEYS:
+                buf = {s.suffix: getattr(module, f"{key}_{s.suffix}", None) for s in STORAGE["mxfp4"]}
+                codes = buf["mxfp4"]
+                dense = (*codes.shape[:2], 2 * codes.shape[2]) if getattr(codes, "ndim", 0) == 3 else ()
+                problems = storage_problems("mxfp4", key, E, dense, None, buf)
+                if problems:
+                    raise ops._lib.MiraiError(2, "MXFP4 expert buffers do not fit the kernel layout: "
+                                              + "; ".join(problems))
+                ws[key] = ops.Mxfp4Tensor(codes, buf["mxfp4_scale"])
+            _, inter, hidden = ws["w1"].shape
+            return cls("mxfp4", ws["w1"], ws["w3"], ws["w2"], E, hidden, inter)
         w1, w2, w3 = (getattr(module, k, None) for k in ("w1", "w2", "w3"))
         if all(isinstance(w, torch.Tensor) for w in (w1, w2, w3)):
             bf = [w.detach().to(torch.bfloat16).contiguous() for w in (w1, w3, w2)]
@@ -350,9 +372,9 @@ class B200GroupedExperts(nn.Module):
         manifest (packed_state.py:331-341, 441-449) and its tensor mapping
         (safetensors names -> tensors, e.g. ``layers.3.ffn.experts.w1_nf4``).
 
-        NF4 and INT8 entries are read; ``spec["tensors"]`` maps each local
-        buffer name (``w1_nf4``, ``w1_nf4_absmax``, ... or ``w1_int8``,
-        ``w1_scale``) to its tensor key, ``spec["shapes"]`` gives each key's
+        NF4, INT8 and MXFP4 entries are read; ``spec["tensors"]`` maps each local
+        buffer name (``w1_nf4``, ``w1_nf4_absmax``, ..., ``w1_int8``,
+        ``w1_scale`` or ``w1_mxfp4``, ``w1_mxfp4_scale``) to its tensor key, ``spec["shapes"]`` gives each key's
         dense shape, ``spec["group_sizes"]`` the INT8 rotation groups and
         ``spec["nf4_meta"]`` the NF4 block sizes.  The tensors must already be
         on the CUDA device that will run the layer (they are used in place)."""
@@ -360,7 +382,7 @@ class B200GroupedExperts(nn.Module):
             raise ValueError(f"packed entry of kind {spec.get('kind')!r} is not grouped_experts")
         fmt = str(spec.get("quant_format", "")).lower()
         if fmt not in STORAGE:
-            raise ValueError(f"packed grouped experts in format {fmt!r}: the fused path reads nf4 and int8")
+            raise ValueError(f"packed grouped experts in format {fmt!r}: the fused path reads nf4, int8 and mxfp4")
         if spec.get("rotations"):
             raise ValueError("packed grouped experts with learned rotations: the fused path applies the fixed "
                              "block-Hadamard rotation only")
@@ -382,6 +404,8 @@ class B200GroupedExperts(nn.Module):
                 m.load_nf4_packed_weight(key, packed=buf["nf4"], absmax=buf["nf4_absmax"],
                                          nested_absmax=buf["nf4_nabsmax"], offset=buf["nf4_offset"],
                                          code=buf["nf4_code"], nested_code=buf["nf4_ncode"], shape=shape, meta=meta)
+            elif fmt == "mxfp4":
+                m.load_mxfp4_weight(key, packed=buf["mxfp4"], scale=buf["mxfp4_scale"])
             else:
                 m.load_quantized_weight(key, weight_int8=buf["int8"], weight_scale=buf["scale"],
                                         group_size=int(groups.get(key, 0)))
@@ -389,8 +413,8 @@ class B200GroupedExperts(nn.Module):
 
     def _init_empty(self, num_experts, quant_format, nf4_blocksize, access, chunk, group_sizes=None):
         fmt = str(quant_format or "nf4").lower()
-        if fmt not in ("nf4", "int8", "bf16"):
-            raise ValueError(f"quant_format {quant_format!r}: the B200 experts store nf4, int8 or bf16")
+        if fmt not in ("nf4", "int8", "mxfp4", "bf16"):
+            raise ValueError(f"quant_format {quant_format!r}: the B200 experts store nf4, int8, mxfp4 or bf16")
         self.num_experts = int(num_experts)
         self._quant_format = fmt
         self._nf4_blocksize = int(nf4_blocksize)
@@ -446,6 +470,9 @@ class B200GroupedExperts(nn.Module):
                                   group_size=g)
             self._install(key, "int8", {"int8": t.q, "scale": t.scale})
             setattr(self, f"{key}_group_size", g)
+        elif self._quant_format == "mxfp4":
+            t = ops.mxfp4_quantize(src if src.dtype in (torch.float32, torch.bfloat16, torch.float16) else src.float())
+            self._install(key, "mxfp4", {"mxfp4": t.packed, "mxfp4_scale": t.scale})
         else:
             self._install(key, "bf16", {"": src.to(torch.bfloat16).contiguous()})
 
@@ -495,6 +522,28 @@ class B200GroupedExperts(nn.Module):
                                     "scale": weight_scale.detach().float().contiguous()})
         setattr(self, f"{key}_group_size", g)
 
+    def load_mxfp4_weight(self, key: str, *, packed: torch.Tensor, scale: torch.Tensor) -> None:
+        """Restore one MXFP4 key: codes uint8 [E, out, in/2] (first element in the
+        low half) and scale bytes uint8, in rows [E, out, in/32] as MX checkpoints
+        store them or in the kernels' tiles [E, ceil(out/128), ceil(in/128), 512]."""
+        self._check_key(key)
+        if self._quant_format != "mxfp4":
+            raise ValueError(f"MXFP4 buffers for {key} offered to {self._quant_format} experts")
+        if packed.ndim != 3:
+            raise ValueError(f"MXFP4 {key} of shape {tuple(packed.shape)}: expected [E, out, in/2]")
+        dense = (*(int(d) for d in packed.shape[:2]), 2 * int(packed.shape[2]))
+        if scale.ndim == 3:
+            if tuple(scale.shape) != (*dense[:2], dense[2] // ops.MXFP4_BLOCK):
+                raise ValueError(f"{key}_mxfp4_scale: rows of shape {tuple(scale.shape)}, expected "
+                                 f"{(*dense[:2], dense[2] // ops.MXFP4_BLOCK)}")
+            scale = ops.mxfp4_scale_tiles(scale)
+        tiles = (dense[0], -(-dense[1] // 128), -(-dense[2] // 128), 512)
+        problems = storage_problems("mxfp4", key, self.num_experts, dense, None, {"mxfp4": packed, "mxfp4_scale": scale})
+        if not problems and tuple(scale.shape) != tiles:
+            problems.append(f"{key}_mxfp4_scale: shape {tuple(scale.shape)}, expected {tiles}")
+        _require(problems, f"MXFP4 buffers for {key}")
+        self._install(key, "mxfp4", {"mxfp4": packed.detach().contiguous(), "mxfp4_scale": scale.detach().contiguous()})
+
     def is_fully_loaded(self) -> bool:
         return self._loaded.issuperset({"w1", "w2", "w3"})
 
@@ -534,6 +583,9 @@ class B200GroupedExperts(nn.Module):
             t = self._buffers.get(name)
             if t is not None:
                 return tuple(t.shape)
+        codes = self._buffers.get(f"{key}_mxfp4")
+        if codes is not None:
+            return (*codes.shape[:2], 2 * codes.shape[2])
         raise RuntimeError(f"{key} is not loaded")
 
     def run_direct_routed(self, tokens: torch.Tensor, top_scores: torch.Tensor,

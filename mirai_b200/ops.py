@@ -277,6 +277,242 @@ def swiglu_backward_rotated(dh_raw: torch.Tensor, gate_up: torch.Tensor, group: 
     return dgu
 
 
+# ----------------------------------------------------------------------------- MXFP4
+
+MXFP4_BLOCK = 32
+_MXFP4_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 3}
+
+
+def _same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call runs on {device}")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` at a 16-byte aligned address (a copy when a view starts elsewhere)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _tiles(rows: int, width: int) -> tuple[int, int]:
+    return -(-rows // 128), -(-width // 128)
+
+
+def mxfp4_scale_tiles(scale: torch.Tensor) -> torch.Tensor:
+    """Scale bytes uint8 [E, out, in/32] (the row order of MX checkpoints) in the
+    tile order the kernels read: [E, ceil(out/128), ceil(in/128), 512]."""
+    if scale.dtype != torch.uint8 or scale.ndim != 3:
+        raise ValueError(f"scale bytes must be uint8 [E, out, in/32], got {scale.dtype} {tuple(scale.shape)}")
+    E, out_f, blocks = scale.shape
+    rt, kt = _tiles(out_f, blocks * MXFP4_BLOCK)
+    full = scale.new_zeros((E, rt * 128, kt * 4))
+    full[:, :out_f, :blocks] = scale
+    return full.view(E, rt, 4, 32, kt, 4).permute(0, 1, 4, 3, 2, 5).reshape(E, rt, kt, 512)
+
+
+def mxfp4_scale_rows(tiles: torch.Tensor, out_features: int, in_features: int) -> torch.Tensor:
+    """The inverse of ``mxfp4_scale_tiles``: scale bytes [E, out, in/32]."""
+    E, rt, kt, _ = tiles.shape
+    rows = tiles.view(E, rt, kt, 32, 4, 4).permute(0, 1, 4, 3, 2, 5).reshape(E, rt * 128, kt * 4)
+    return rows[:, :out_features, :in_features // MXFP4_BLOCK].contiguous()
+
+
+class Mxfp4Tensor:
+    """Device buffers of one MXFP4 grouped-expert key [E, out, in]: ``packed``
+    uint8 [E, out, in/2] (two E2M1 codes per byte, the first element in the low
+    half) and ``scale`` uint8 [E, ceil(out/128), ceil(in/128), 512], a
+    power-of-two exponent byte per 32 elements of a row, in tiles
+    (``mxfp4_scale_tiles`` makes them of a checkpoint's [E, out, in/32])."""
+
+    def __init__(self, packed: torch.Tensor, scale: torch.Tensor):
+        self.packed = _aligned(_cuda(packed, "packed", torch.uint8))
+        self.scale = _aligned(_cuda(scale, "scale", torch.uint8))
+        if self.packed.ndim != 3 or self.packed.shape[2] % (MXFP4_BLOCK // 2) or 0 in self.packed.shape:
+            raise ValueError(f"MXFP4 codes must be [E, out, in/2] with in % 32 == 0, got {tuple(self.packed.shape)}")
+        E, out_f, half = self.packed.shape
+        want = (E, *_tiles(out_f, 2 * half), 512)
+        if tuple(self.scale.shape) != want:
+            raise ValueError(f"MXFP4 scale tiles of shape {tuple(self.scale.shape)}: {E} x {out_f} x {2 * half} needs "
+                             f"{want}")
+        _same_device(self.packed.device, scale=self.scale)
+        self.shape = (E, out_f, 2 * half)
+        self._struct = _lib.Mxfp4Weight(self.packed.data_ptr(), self.scale.data_ptr())
+
+    def struct(self) -> _lib.Mxfp4Weight:
+        return self._struct
+
+
+class Mxfp4Rows:
+    """Activation rows [S, width] in MXFP4, grouped in ``segments`` segments (one
+    per expert, or per source and expert): ``packed`` uint8 [S, width/2] and
+    ``scale`` uint8 [tiles, ceil(width/128), 512], whose row tiles restart at
+    every segment.  Made by ``mxfp4_quantize_rows`` or ``gateup_swiglu(...,
+    quantize=True)``, taken by ``gateup_swiglu`` / ``down`` with the same offsets."""
+
+    def __init__(self, packed: torch.Tensor, scale: torch.Tensor, segments: int):
+        self.packed = _cuda(packed, "packed", torch.uint8)
+        self.scale = _cuda(scale, "scale", torch.uint8)
+        if self.packed.ndim != 2 or self.packed.shape[1] == 0 or self.packed.shape[1] % (MXFP4_BLOCK // 2):
+            raise ValueError(f"MXFP4 rows must be [S, width/2] with width % 32 == 0, got {tuple(self.packed.shape)}")
+        self.segments = int(segments)
+        self.shape = (self.packed.shape[0], 2 * self.packed.shape[1])
+        self.device = self.packed.device
+        need = self.scale_bytes(*self.shape, self.segments)
+        if self.segments < 1 or self.scale.numel() < need:
+            raise ValueError(f"{self.shape[0]} rows of {self.shape[1]} in {self.segments} segments need {need} scale "
+                             f"bytes, got {self.scale.numel()}")
+        _same_device(self.device, scale=self.scale)
+        if self.packed.data_ptr() % 16 or self.scale.data_ptr() % 16:
+            raise ValueError("MXFP4 rows must start 16-byte aligned")
+
+    @staticmethod
+    def scale_bytes(rows: int, width: int, segments: int) -> int:
+        return int(_lib.load().mirai_mxfp4_rows_scale_bytes(rows, segments, width))
+
+    @classmethod
+    def empty(cls, rows: int, width: int, segments: int, device) -> "Mxfp4Rows":
+        kt = _tiles(0, width)[1]
+        tiles = cls.scale_bytes(rows, width, segments) // (512 * kt)
+        return cls(torch.empty((rows, width // 2), dtype=torch.uint8, device=device),
+                   torch.empty((tiles, kt, 512), dtype=torch.uint8, device=device), segments)
+
+
+def mxfp4_quantize(weight: torch.Tensor) -> Mxfp4Tensor:
+    """Quantise a [E, out, in] stack (bf16, fp32 or fp16) to MXFP4: per 32 elements
+    of a row the scale 2^(floor(log2 max|x|) - 2), elements rounded to the
+    nearest E2M1 value (ties to even, saturating).  A block holding an infinity
+    or a NaN reads back as NaN."""
+    w = _aligned(_cuda(weight, "weight"))
+    if w.dtype not in _MXFP4_DTYPES:
+        raise TypeError(f"mxfp4_quantize takes bf16, fp32 or fp16, got {w.dtype}")
+    if w.ndim != 3 or 0 in w.shape or w.shape[2] % MXFP4_BLOCK:
+        raise ValueError(f"mxfp4_quantize takes [E, out, in] with in % 32 == 0, got {tuple(w.shape)}")
+    E, out_f, in_f = w.shape
+    packed = torch.empty((E, out_f, in_f // 2), dtype=torch.uint8, device=w.device)
+    # rows past `out` in the last tile are zero bytes too
+    make = torch.empty if out_f % 128 == 0 else torch.zeros
+    scale = make((E, *_tiles(out_f, in_f), 512), dtype=torch.uint8, device=w.device)
+    with torch.cuda.device(w.device):
+        _lib.call("mirai_mxfp4_quantize", _ptr(w), _MXFP4_DTYPES[w.dtype], E, out_f, in_f, _ptr(packed), _ptr(scale),
+                  _stream())
+    return Mxfp4Tensor(packed, scale)
+
+
+def mxfp4_dequantize(w: Mxfp4Tensor, out: torch.Tensor | None = None,
+                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The [E, out, in] values of an MXFP4 key, exact in bf16 and fp32 (fp16: rounded
+    to nearest)."""
+    if not isinstance(w, Mxfp4Tensor):
+        raise TypeError(f"mxfp4_dequantize reads an Mxfp4Tensor, not {type(w)}")
+    if out is None:
+        if out_dtype not in _MXFP4_DTYPES:
+            raise TypeError(f"mxfp4_dequantize writes bf16, fp32 or fp16, not {out_dtype}")
+        out = torch.empty(w.shape, dtype=out_dtype, device=w.packed.device)
+    if out.dtype not in _MXFP4_DTYPES or tuple(out.shape) != w.shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {w.shape} tensor of bf16, fp32 or fp16, got {out.dtype} "
+                         f"{tuple(out.shape)}")
+    _same_device(w.packed.device, out=out)
+    E, out_f, in_f = w.shape
+    with torch.cuda.device(out.device):
+        _lib.call("mirai_mxfp4_dequantize", _ptr(w.packed), _ptr(w.scale), E, out_f, in_f, _ptr(out),
+                  _MXFP4_DTYPES[out.dtype], _stream())
+    return out
+
+
+def mxfp4_quantize_rows(x: torch.Tensor, offsets: torch.Tensor, row_index: torch.Tensor | None = None) -> Mxfp4Rows:
+    """bf16 rows [S, width] of the segments ``offsets`` ends (int32), quantised for
+    the expert products.  ``row_index`` int64 [S]: row s is x[row_index[s]] (the
+    permute in the same pass).  Rows past the last segment are not written."""
+    x = _aligned(_cuda(x, "x", torch.bfloat16))
+    offsets = _cuda(offsets, "offsets", torch.int32)
+    if x.ndim != 2 or x.shape[1] % MXFP4_BLOCK or x.shape[1] == 0:
+        raise ValueError(f"mxfp4_quantize_rows takes [rows, width] with width % 32 == 0, got {tuple(x.shape)}")
+    index = None if row_index is None else _cuda(row_index, "row_index", torch.int64)
+    _same_device(x.device, offsets=offsets, row_index=index)
+    S = x.shape[0] if index is None else index.numel()
+    rows = Mxfp4Rows.empty(S, x.shape[1], offsets.numel(), x.device)
+    with torch.cuda.device(x.device):
+        _lib.call("mirai_mxfp4_quantize_rows", _ptr(x), x.shape[0], _ptr(index), _ptr(offsets), offsets.numel(), S,
+                  x.shape[1], _ptr(rows.packed), _ptr(rows.scale), _stream())
+    return rows
+
+
+def _mxfp4_rows(x, offsets: torch.Tensor, width: int, name: str) -> Mxfp4Rows:
+    rows = x if isinstance(x, Mxfp4Rows) else mxfp4_quantize_rows(x, offsets)
+    if rows.shape[1] != width or rows.segments != offsets.numel():
+        raise ValueError(f"{name} of width {rows.shape[1]} in {rows.segments} segments: the call needs width {width} in "
+                         f"{offsets.numel()}")
+    return rows
+
+
+def _mxfp4_output(out: torch.Tensor | None, shape: tuple, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or not out.is_contiguous() or out.device != device:
+        raise ValueError(f"out must be a contiguous bf16 {shape} tensor on {device}, got {out.dtype} "
+                         f"{tuple(out.shape)} on {out.device}")
+    return out
+
+
+def _gateup_mxfp4(x, offsets: torch.Tensor, w1: Mxfp4Tensor, w3: Mxfp4Tensor, *, inter: int, save_gate_up: bool,
+                  want_h: bool, want_rows: bool, out: torch.Tensor | None = None, sources: int = 1):
+    """(h or None, gate_up or None, quantised h or None)."""
+    if not isinstance(w1, Mxfp4Tensor) or not isinstance(w3, Mxfp4Tensor) or w1.shape != w3.shape:
+        raise TypeError("gate/up in MXFP4 needs two Mxfp4Tensor keys of one shape")
+    E, out_f, hidden = w1.shape
+    offsets = _cuda(offsets, "offsets", torch.int32)
+    if out_f != inter or offsets.numel() != sources * E:
+        raise ValueError(f"keys of {E} experts x {out_f} channels: the call has inter {inter} and {offsets.numel()} "
+                         f"segments of {sources} source(s)")
+    device = w1.packed.device
+    _same_device(device, x=x, offsets=offsets, w3=w3.packed)
+    rows = _mxfp4_rows(x, offsets, hidden, "x_sorted")
+    S = rows.shape[0]
+    h = _mxfp4_output(out, (S, inter), device) if want_h else None
+    gu = torch.empty((S, 2 * inter), dtype=torch.bfloat16, device=device) if save_gate_up else None
+    hq = Mxfp4Rows.empty(S, inter, offsets.numel(), device) if want_rows else None
+    with torch.cuda.device(device):
+        _lib.call("mirai_moe_gateup_swiglu_mxfp4", _ptr(rows.packed), _ptr(rows.scale), _ptr(offsets), sources, E, S,
+                  hidden, inter, w1.struct(), w3.struct(), _ptr(h), _ptr(gu), _ptr(hq.packed if hq else None),
+                  _ptr(hq.scale if hq else None), _stream())
+    return h, gu, hq
+
+
+def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: torch.Tensor | None,
+                lora: "DownLoRA | None", rank_a: torch.Tensor | None, sources: int) -> torch.Tensor:
+    E, out_f, inter = w2.shape
+    offsets = _cuda(offsets, "offsets", torch.int32)
+    if out_f != hidden or offsets.numel() != sources * E:
+        raise ValueError(f"a key of {E} experts x {out_f} rows: the call has hidden {hidden} and {offsets.numel()} "
+                         f"segments of {sources} source(s)")
+    device = w2.packed.device
+    _same_device(device, h=h, offsets=offsets, rank_a=rank_a)
+    low = rank_b = None
+    if lora is not None:
+        if rank_a is None and isinstance(h, Mxfp4Rows):
+            raise ValueError("a LoRA adapter on quantised rows needs rank_a, its projection of the bf16 rows")
+        low = rank_a if rank_a is not None else lora_project(h, offsets, lora, forward=True, sources=sources)
+        if tuple(low.shape) != (h.shape[0], 64) or low.dtype != torch.bfloat16 or not low.is_contiguous():
+            raise ValueError(f"rank_a must be contiguous bf16 [{h.shape[0]}, 64], got {low.dtype} {tuple(low.shape)}")
+        rank_b = lora.b_pad()
+        if rank_b.shape[0] != E * hidden:
+            raise ValueError(f"the adapter's B has {rank_b.shape[0]} rows, the key {E} x {hidden}")
+        _same_device(device, lora=rank_b)
+    rows = _mxfp4_rows(h, offsets, inter, "h")
+    S = rows.shape[0]
+    y = _mxfp4_output(out, (S, hidden), device)
+    with torch.cuda.device(device):
+        _lib.call("mirai_moe_down_mxfp4", _ptr(rows.packed), _ptr(rows.scale), _ptr(offsets), sources, E, S, inter, hidden,
+                  w2.struct(), _ptr(low), _ptr(rank_b), _ptr(y), _stream())
+    return y
+
+
+def _dx_weight(w):
+    """The weight a dX product multiplies: an MXFP4 key is read back (the scales run
+    along the other axis than dX reduces over), others as given."""
+    return mxfp4_dequantize(w) if isinstance(w, Mxfp4Tensor) else w
+
+
 def _group(w) -> int:
     return int(getattr(w, "group_size", 0) or 0)
 
@@ -290,11 +526,26 @@ def _as_weight(w):
 # ----------------------------------------------------------------------------- a6 / a7
 
 def gateup_swiglu(x_sorted: torch.Tensor, offsets: torch.Tensor, w1, w3, *, inter: int,
-                  save_gate_up: bool = False, out: torch.Tensor | None = None, sources: int = 1):
+                  save_gate_up: bool = False, out: torch.Tensor | None = None, sources: int = 1,
+                  quantize: bool = False):
     """h = silu(x W1^T) * (x W3^T) per expert segment.  ``w1``/``w3`` are bf16
     tensors [E, I, H], or ``Nf4Weight`` / ``Int8Weight`` descriptors.
     ``sources`` > 1: ``offsets`` ends ``sources * E`` source-major segments
-    (segment s*E + e = source s's rows for expert e)."""
+    (segment s*E + e = source s's rows for expert e).
+
+    ``Mxfp4Tensor`` keys multiply the rows in MXFP4 too: ``x_sorted`` is bf16
+    (quantised here) or ``Mxfp4Rows``; silu(g) * u is formed in fp32 and rounded
+    once, and ``quantize=True`` returns h as the ``Mxfp4Rows`` that ``down``
+    takes instead of bf16."""
+    if isinstance(w1, Mxfp4Tensor) or isinstance(w3, Mxfp4Tensor):
+        if quantize and out is not None:
+            raise ValueError("quantize=True returns Mxfp4Rows: it writes no bf16 out")
+        h, gu, hq = _gateup_mxfp4(x_sorted, offsets, w1, w3, inter=inter, save_gate_up=save_gate_up,
+                                  want_h=not quantize, want_rows=quantize, out=out, sources=sources)
+        h = hq if quantize else h
+        return (h, gu) if save_gate_up else h
+    if quantize:
+        raise TypeError("quantize=True needs MXFP4 keys")
     w1, w3 = _as_weight(w1), _as_weight(w3)
     x_sorted = _cuda(x_sorted, "x_sorted", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
@@ -329,7 +580,10 @@ def down(h: torch.Tensor, offsets: torch.Tensor, w2, *, hidden: int, out: torch.
          lora: "DownLoRA | None" = None, rank_a: torch.Tensor | None = None, sources: int = 1):
     """y = h W2^T per expert segment (+ the fused LoRA rank block when ``lora``;
     ``rank_a`` is its [S, 64] projection of h when the caller already has it).
-    ``sources`` > 1: source-major segments as in ``gateup_swiglu``."""
+    ``sources`` > 1: source-major segments as in ``gateup_swiglu``.  With an
+    ``Mxfp4Tensor`` key, ``h`` is bf16 (quantised here) or ``Mxfp4Rows``."""
+    if isinstance(w2, Mxfp4Tensor):
+        return _down_mxfp4(h, offsets, w2, hidden=hidden, out=out, lora=lora, rank_a=rank_a, sources=sources)
     w2 = _as_weight(w2)
     h = _cuda(h, "h", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
@@ -515,7 +769,7 @@ def down_dx(grad_y: torch.Tensor, offsets: torch.Tensor, w2, gate_up: torch.Tens
     source-major segments (an expert owner's rows); there ``gate_up=None``
     returns dh [S, I] itself."""
     group = getattr(w2, "group_size", 0)  # block-Hadamard INT8: the rotation group of dh
-    w2 = _as_weight(w2)
+    w2 = _as_weight(_dx_weight(w2))
     gy = _cuda(grad_y, "grad_y", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
     S, H = gy.shape
@@ -590,7 +844,7 @@ def gateup_dx(grad_gate_up: torch.Tensor, offsets: torch.Tensor, w1, w3, *, hidd
               out: torch.Tensor | None = None, sources: int = 1) -> torch.Tensor:
     """dx_sorted [S, H] = dgate W1 + dup W3 per expert segment (``sources`` > 1:
     source-major segments)."""
-    w1, w3 = _as_weight(w1), _as_weight(w3)
+    w1, w3 = _as_weight(_dx_weight(w1)), _as_weight(_dx_weight(w3))
     dgu = _cuda(grad_gate_up, "grad_gate_up", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
     S, I2 = dgu.shape
@@ -682,7 +936,12 @@ def moe_forward(tokens: torch.Tensor, top_indices: torch.Tensor, top_weights: to
 
     Rotated INT8 weights: the tokens are rotated before the permute (T rows,
     not S) and h before the down GEMM; the LoRA rank block is projected from
-    the unrotated h."""
+    the unrotated h.  MXFP4 weights: the tokens are quantised as they are
+    permuted, and h as it is formed."""
+    if any(isinstance(w, Mxfp4Tensor) for w in (w1, w3, w2)):
+        plan = dispatch_plan(top_indices, num_experts)
+        y = _mxfp4_experts(tokens, plan, w1, w3, w2, inter=inter, lora=lora, train=False)[0]
+        return combine(y, plan.inverse_order, top_weights, out_dtype=out_dtype or tokens.dtype)
     g_in, g_mid = _rotations(w1, w3, w2)
     (w1, w3, w2), join = _stage_beside((w1, w3, w2), top_indices.numel(), num_experts, training=False)
     plan = dispatch_plan(top_indices, num_experts)
@@ -693,6 +952,19 @@ def moe_forward(tokens: torch.Tensor, top_indices: torch.Tensor, top_weights: to
     y = down(rotate_rows(h, g_mid) if g_mid else h, plan.offsets, w2, hidden=tokens.shape[1], lora=lora,
              rank_a=low)
     return combine(y, plan.inverse_order, top_weights, out_dtype=out_dtype or tokens.dtype)
+
+
+def _mxfp4_experts(tokens, plan: DispatchPlan, w1, w3, w2, *, inter: int, lora: DownLoRA | None, train: bool):
+    """(y, gate_up, h, rank_a) of the routed rows in MXFP4: quantised in the
+    permute's pass, h in the gate/up epilogue.  gate_up when ``train``; h and
+    rank_a with a LoRA adapter, whose projection reads h in bf16."""
+    if not all(isinstance(w, Mxfp4Tensor) for w in (w1, w3, w2)):
+        raise TypeError("MXFP4 experts hold all three keys in MXFP4")
+    rows = mxfp4_quantize_rows(tokens, plan.offsets, row_index=plan.sorted_token_indices)
+    h, gu, hq = _gateup_mxfp4(rows, plan.offsets, w1, w3, inter=inter, save_gate_up=train, want_h=lora is not None,
+                              want_rows=True)
+    low = lora_project(h, plan.offsets, lora, forward=True) if lora is not None else None
+    return down(hq, plan.offsets, w2, hidden=tokens.shape[1], lora=lora, rank_a=low), gu, h, low
 
 
 @dataclass
@@ -786,6 +1058,12 @@ def _stage_beside(weights, rows: int, num_experts: int, *, training: bool):
 def moe_forward_train(tokens, top_indices, top_weights, w1, w3, w2, *, num_experts: int, inter: int,
                       out_dtype: torch.dtype | None = None, lora: DownLoRA | None = None):
     """Forward that also returns the state the dX pass consumes."""
+    if any(isinstance(w, Mxfp4Tensor) for w in (w1, w3, w2)):
+        plan = dispatch_plan(top_indices, num_experts)
+        y, gu, h, low = _mxfp4_experts(tokens, plan, w1, w3, w2, inter=inter, lora=lora, train=True)
+        out = combine(y, plan.inverse_order, top_weights, out_dtype=out_dtype or tokens.dtype)
+        keep = lora is not None and lora.compute_grads
+        return out, ForwardState(plan, y, gu, top_weights.float(), h if keep else None, low if keep else None)
     g_in, g_mid = _rotations(w1, w3, w2)
     keys = (w1, w3, w2)
     (w1, w3, w2), join = _stage_beside(keys, top_indices.numel(), num_experts, training=True)
