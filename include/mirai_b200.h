@@ -517,6 +517,29 @@ int mirai_moe_down_dh_lora_int8(const void* grad_y, const int32_t* offsets, int3
 int mirai_swiglu_backward_rotated(const void* dh, const void* gate_up, int64_t rows, int32_t inter, int32_t group,
                                   void* grad_gate_up, mirai_stream_t stream);
 
+/* ------------------------------------------------ group-limited routing
+ * Experts in num_groups contiguous groups of one size (1..32 groups, E <= 1024): the
+ * top_groups groups with the best score stay (the largest key of a group, or with group_top2
+ * the sum of its two largest score + bias), and of their experts the top_k <= 16 with the
+ * largest key are chosen, in descending order.  Key: score + choice_bias [E], or without a bias
+ * the logit.  Weights: the scores without the bias, renormalised as in mirai_route_topk.
+ * Ties go to the lowest id.  Comparisons come out as in 64-bit arithmetic.  An expert whose logit
+ * is -inf or NaN ranks last whatever its bias and scores 0 (a row of -inf: the lowest ids, weights
+ * 0); a NaN makes its row's weights NaN.  logits_dtype MIRAI_DTYPE_F32 or _BF16.
+ *
+ * The backward writes the whole of grad_logits [T, E] (logits_dtype) from the gradient of the
+ * weights fp32 [T, k] and the chosen ids (an id given twice counts twice; one outside [0, E) is
+ * recorded and skipped).  The reference's routers leave this to autograd
+ * (transformer_lingbot_video.py:1002-1033). */
+int mirai_route_groups(const void* logits, int32_t logits_dtype, int64_t num_tokens, int32_t num_experts, int32_t top_k,
+                       int32_t num_groups, int32_t top_groups, int32_t group_top2, int32_t score_func,
+                       const float* choice_bias, int32_t norm_mode, float route_scale, int64_t* top_indices,
+                       float* top_weights, mirai_stream_t stream);
+int mirai_route_groups_backward(const float* grad_weights, const void* logits, int32_t logits_dtype,
+                                const int64_t* top_indices, int64_t num_tokens, int32_t num_experts, int32_t top_k,
+                                int32_t score_func, int32_t norm_mode, float route_scale, void* grad_logits,
+                                mirai_stream_t stream);
+
 /* ------------------------------------------------ MXFP4 (microscaled 4-bit)
  * Blocks of 32 consecutive elements of a row share the scale 2^e,
  * e = clamp(floor(log2 max|x|) - 2, -127, 127), stored as the byte e + 127; an

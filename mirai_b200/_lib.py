@@ -170,6 +170,10 @@ SIGNATURES = {
                                               c_vp, c_vp]),
     "mirai_moe_down_dh_lora_int8": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i64, c_i32, c_i32,
                                                    ctypes.POINTER(Int8Weight), c_vp, c_vp, c_vp, c_vp]),
+    "mirai_route_groups": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_i32,
+                                          c_f32, c_vp, c_vp, c_vp]),
+    "mirai_route_groups_backward": (ctypes.c_int, [c_vp, c_vp, c_i32, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_f32,
+                                                   c_vp, c_vp]),
     "mirai_mxfp4_scale_bytes": (c_size, [c_i32, c_i64, c_i64]),
     "mirai_mxfp4_rows_scale_bytes": (c_size, [c_i64, c_i32, c_i32]),
     "mirai_mxfp4_quantize": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i64, c_i64, c_vp, c_vp, c_vp]),

@@ -160,15 +160,42 @@ class TokenChunkPolicy:
 
 # ----------------------------------------------------------------------------- router
 
+class _GroupRouteFunction(torch.autograd.Function):
+    """``ops.route_groups`` with its gradient kernel: (ids, fp32 weights) of logits [T, E]."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, top_k, options, weighting):
+        idx, w = ops.route_groups(logits, top_k, choice_bias=bias, **options, **weighting)
+        ctx.save_for_backward(logits, idx)
+        ctx.weighting = weighting
+        ctx.mark_non_differentiable(idx)
+        return idx, w
+
+    @staticmethod
+    def backward(ctx, _, grad_w):
+        logits, idx = ctx.saved_tensors
+        grad = ops.route_groups_backward(grad_w.float(), logits, idx, **ctx.weighting)
+        return grad, None, None, None, None
+
+
 def route(tokens: torch.Tensor, weight: torch.Tensor, *, top_k: int, score_func: str = "sigmoid",
-          correction_bias: torch.Tensor | None = None, norm_topk_prob: bool = True, route_scale: float = 1.0):
+          correction_bias: torch.Tensor | None = None, norm_topk_prob: bool = True, route_scale: float = 1.0,
+          num_groups: int = 1, top_groups: int = 1, group_score: str = "top2"):
     """The LingBot router (transformer_lingbot_video.py:962-1033, without the
     research extensions): returns (top_indices int64 [T, k], top_scores in the
     tokens' dtype).  Selection runs in the sm_100a router kernel on fp32 logits;
     when the router weight needs a gradient the weights are re-gathered in torch
-    from the unbiased scores so that autograd reaches it."""
+    from the unbiased scores so that autograd reaches it.
+
+    ``num_groups`` > 1 limits a token's experts to its ``top_groups`` best groups
+    (``ops.route_groups``, with the gradient in its own kernel)."""
     logits = F.linear(tokens.float(), weight.float())
     bias = None if correction_bias is None else correction_bias.float().contiguous()
+    if num_groups > 1:
+        options = {"num_groups": num_groups, "top_groups": top_groups, "group_score": group_score}
+        weighting = {"score_func": score_func, "norm": "eps" if norm_topk_prob else "none", "route_scale": route_scale}
+        idx, w = _GroupRouteFunction.apply(logits, bias, top_k, options, weighting)
+        return idx, w.to(tokens.dtype)
     lg = logits.detach().contiguous()
     if norm_topk_prob:  # w / (sum w + 1e-20) for k > 1, then * route_scale, in the kernel
         idx, w = ops.route_topk(lg, top_k, score_func=score_func, choice_bias=bias, norm="eps",
@@ -196,10 +223,16 @@ class B200SparseMoeBlock(nn.Module):
 
     def __init__(self, *, hidden_size: int, num_experts: int, top_k: int, score_func: str = "sigmoid",
                  norm_topk_prob: bool = True, route_scale: float = 1.0, experts: nn.Module,
-                 shared_experts: nn.Module | None = None, token_chunk_policy: TokenChunkPolicy | None = None):
+                 shared_experts: nn.Module | None = None, token_chunk_policy: TokenChunkPolicy | None = None,
+                 num_groups: int = 1, top_groups: int = 1, group_score: str = "top2"):
         super().__init__()
         if score_func not in ("sigmoid", "softmax"):
             raise ValueError(f"score_func {score_func!r}: sigmoid or softmax")
+        if num_groups < 1 or num_experts % num_groups or not 1 <= top_groups <= num_groups:
+            raise ValueError(f"{top_groups} of {num_groups} groups of {num_experts} experts")
+        if group_score not in ops.GROUP_SCORES:
+            raise ValueError(f"group_score {group_score!r}: one of {sorted(ops.GROUP_SCORES)}")
+        self.num_groups, self.top_groups, self.group_score = int(num_groups), int(top_groups), group_score
         self.hidden_size, self.num_experts, self.top_k = int(hidden_size), int(num_experts), int(top_k)
         self.score_func, self.norm_topk_prob, self.route_scale = score_func, bool(norm_topk_prob), float(route_scale)
         self.router_weight = nn.Parameter(torch.empty(num_experts, hidden_size))
@@ -212,7 +245,8 @@ class B200SparseMoeBlock(nn.Module):
     @classmethod
     def from_state(cls, state: Mapping[str, torch.Tensor], *, top_k: int, score_func: str = "sigmoid",
                    norm_topk_prob: bool = True, route_scale: float = 1.0,
-                   token_chunk_policy: TokenChunkPolicy | None = None) -> "B200SparseMoeBlock":
+                   token_chunk_policy: TokenChunkPolicy | None = None, num_groups: int = 1, top_groups: int = 1,
+                   group_score: str = "top2") -> "B200SparseMoeBlock":
         """A block from a reference block's state dict: ``router.weight``,
         ``router.e_score_correction_bias``, ``experts.w1/w2/w3`` (dense, or the
         experts module passed already quantised as ``state["experts"]``) and,
@@ -233,7 +267,8 @@ class B200SparseMoeBlock(nn.Module):
                                     if k.startswith("shared_experts.")})
         blk = cls(hidden_size=H, num_experts=E, top_k=top_k, score_func=score_func, norm_topk_prob=norm_topk_prob,
                   route_scale=route_scale, experts=experts, shared_experts=shared,
-                  token_chunk_policy=token_chunk_policy).to(rw.device)
+                  token_chunk_policy=token_chunk_policy, num_groups=num_groups, top_groups=top_groups,
+                  group_score=group_score).to(rw.device)
         with torch.no_grad():
             blk.router_weight.copy_(rw)
             if "router.e_score_correction_bias" in state:
@@ -249,7 +284,8 @@ class B200SparseMoeBlock(nn.Module):
         tokens = hidden_states.reshape(-1, self.hidden_size)
         idx, scores = route(tokens, self.router_weight, top_k=self.top_k, score_func=self.score_func,
                             correction_bias=self.e_score_correction_bias, norm_topk_prob=self.norm_topk_prob,
-                            route_scale=self.route_scale)
+                            route_scale=self.route_scale, num_groups=self.num_groups, top_groups=self.top_groups,
+                            group_score=self.group_score)
         if padding_mask is not None:  # transformer_lingbot_video.py:2283-2287
             pm = padding_mask.reshape(-1, 1).to(scores.dtype)
             scores = scores * pm

@@ -9,3 +9,4 @@
 #include "exchange.cu"
 #include "rotate.cu"
 #include "mxfp4.cu"
+#include "route_groups.cu"

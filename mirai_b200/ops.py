@@ -86,6 +86,75 @@ def route_topk(logits: torch.Tensor, top_k: int, *, score_func: str = "softmax",
     return idx, w
 
 
+GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+def _route_options(score_func: str, norm: str) -> tuple[int, int]:
+    if score_func not in SCORE_FUNCS:
+        raise ValueError(f"score_func {score_func!r}: one of {sorted(SCORE_FUNCS)}")
+    if norm not in NORM_MODES:
+        raise ValueError(f"norm {norm!r}: one of {sorted(NORM_MODES)}")
+    return SCORE_FUNCS[score_func], NORM_MODES[norm]
+
+
+def _route_logits(logits: torch.Tensor) -> torch.Tensor:
+    logits = _cuda(logits, "logits")
+    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.ndim != 2:
+        raise TypeError(f"logits must be fp32 or bf16 [T, E], got {logits.dtype} {tuple(logits.shape)}")
+    return logits
+
+
+def route_groups(logits: torch.Tensor, top_k: int, *, num_groups: int = 1, top_groups: int = 1,
+                 group_score: str = "top2", score_func: str = "sigmoid", choice_bias: torch.Tensor | None = None,
+                 norm: str = "eps", route_scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Group-limited top-k routing of fp32 or bf16 logits [T, E]: of ``num_groups``
+    contiguous groups of experts the ``top_groups`` best stay (``group_score``:
+    "max", a group's largest key, or "top2", the sum of its two largest score +
+    bias), and of their experts the ``top_k`` with the largest score + bias (the
+    largest logits without a bias).  Weights are the scores without the bias,
+    renormalised as in ``route_topk``.
+
+    Returns (top_indices int64 [T, k], top_weights fp32 [T, k]) in descending
+    choice order, ties to the lower expert id; comparisons come out as in
+    64-bit arithmetic.  An expert whose logit is -inf or NaN ranks last,
+    whatever its bias; a NaN makes its row's weights NaN."""
+    score, mode = _route_options(score_func, norm)
+    if group_score not in GROUP_SCORES:
+        raise ValueError(f"group_score {group_score!r}: one of {sorted(GROUP_SCORES)}")
+    logits = _route_logits(logits)
+    T, E = logits.shape
+    bias = None if choice_bias is None else _cuda(choice_bias, "choice_bias", torch.float32)
+    if bias is not None and tuple(bias.shape) != (E,):
+        raise ValueError(f"choice_bias of shape {tuple(bias.shape)} for {E} experts")
+    _same_device(logits.device, choice_bias=bias)
+    idx = torch.empty((T, max(int(top_k), 0)), dtype=torch.int64, device=logits.device)
+    w = torch.empty((T, max(int(top_k), 0)), dtype=torch.float32, device=logits.device)
+    with torch.cuda.device(logits.device):
+        _lib.call("mirai_route_groups", _ptr(logits), _DTYPE_CODES[logits.dtype], T, E, top_k, num_groups, top_groups,
+                  GROUP_SCORES[group_score], score, _ptr(bias), mode, float(route_scale), _ptr(idx), _ptr(w), _stream())
+    return idx, w
+
+
+def route_groups_backward(grad_weights: torch.Tensor, logits: torch.Tensor, top_indices: torch.Tensor, *,
+                          score_func: str = "sigmoid", norm: str = "eps", route_scale: float = 1.0) -> torch.Tensor:
+    """Gradient of ``route_groups``' weights with respect to the logits, [T, E] in
+    the logits' dtype, from the gradient of the weights fp32 [T, k] and the
+    chosen ids (the choice itself carries no gradient; the bias neither)."""
+    score, mode = _route_options(score_func, norm)
+    logits = _route_logits(logits)
+    idx = _cuda(top_indices, "top_indices", torch.int64)
+    gw = _cuda(grad_weights, "grad_weights", torch.float32)
+    T, E = logits.shape
+    if idx.ndim != 2 or idx.shape[0] != T or gw.shape != idx.shape:
+        raise ValueError(f"grad_weights {tuple(gw.shape)} and top_indices {tuple(idx.shape)} for {T} tokens")
+    _same_device(logits.device, grad_weights=gw, top_indices=idx)
+    grad = torch.empty_like(logits)
+    with torch.cuda.device(logits.device):
+        _lib.call("mirai_route_groups_backward", _ptr(gw), _ptr(logits), _DTYPE_CODES[logits.dtype], _ptr(idx), T, E,
+                  idx.shape[1], score, mode, float(route_scale), _ptr(grad), _stream())
+    return grad
+
+
 # ----------------------------------------------------------------------------- a2
 
 @dataclass(frozen=True)
