@@ -298,37 +298,46 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 // A tile is 256 rows of one segment x 256 accumulator columns (128 channels of
 // gate beside the same 128 of up, or 256 output columns), on a CTA pair
 // (cta_group::2, M = 256): each SM stages its own 128 rows of A and half of B.
-// A stage is 256 elements of K: 128-byte rows of codes (128-byte swizzle, one
-// TMA box per operand) and the scale tiles of both operands (two 512-byte
-// tiles per 128 rows), which tcgen05.cp puts into TMEM right before the
-// stage's four K = 64 MMAs.  Every SM holds the scales of all 256 columns.
+// A k-block is 256 elements of K: 128-byte rows of codes (128-byte swizzle, one
+// TMA box per operand) and the scale tiles of both operands.
 //
-// TMEM: two 256-column accumulators plus the scales do not fit 512 columns, so
-// the accumulators overlap by 64 columns (0..255 and 192..447): the epilogue
-// reads the shared 64 first and then lets the next tile's MMAs start.
+// What bounds it: at the fp4 rate a pair's 256 x 256 tile takes 512 cycles per
+// k-block, in which streaming both operands would move 32 KB to each SM, more
+// than L2 delivers (loads alone took 127 us of the 32768-token layer's gate/up,
+// the MMAs 91).  So a pair keeps the A rows of a row tile in shared memory
+// (up to 8 k-blocks, K <= 2048; longer rows are streamed) and walks over a run of
+// column tiles, streaming B.  The scales go to TMEM by tcgen05.st from four
+// warps instead of tcgen05.cp, whose copies occupy the tensor pipe (49 us of
+// the same product).
 //
-// Warps: 0 TMA producer, 1 MMA issuer (the leader CTA's), 4..11 epilogue (two
-// per TMEM lane quarter).
+// TMEM: one 256-column accumulator and eight 32-column slots of scales (8 columns
+// for A, 16 for B, one slot per B stage).  The epilogue warps read the whole
+// accumulator at once, release it, and finish from registers while the next
+// tile's MMAs run.
+//
+// Warps: 0 TMA producer of codes, 1 MMA issuer (the leader CTA's), 2 TMA producer of
+// scales, 4..7 scales to TMEM, 8..15 epilogue (two per TMEM lane quarter).
 enum Mode { GATEUP = 0, DOWN = 1 };
 
 constexpr int BM = 128;
 constexpr int TILE_M = 2 * BM;
 constexpr int TN = 256;
-constexpr int BKE = 256;  // elements of K per stage
-constexpr int STAGES = 5;
+constexpr int BKE = 256;           // elements of K per k-block
+constexpr int A_BUFS = 8;          // most k-blocks of A in shared memory
+constexpr int B_STAGES = 8;        // most stages of B (and TMEM scale slots)
 constexpr uint32_t A_BYTES = BM * 128;
 constexpr uint32_t B_BYTES = (TN / 2) * 128;
-constexpr uint32_t SFA_BYTES = 1024;      // two K tiles of this CTA's 128 rows
-constexpr uint32_t SFB_BYTES = 2 * 1024;  // two K tiles of both 128-column halves
-constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-constexpr int EPI_WARPS = 8;
-constexpr int EPI_FIRST = 4;
+constexpr uint32_t SF_BYTES = 3 * 1024;  // two K tiles of this CTA's 128 rows and of both 128-column halves
+constexpr int SF_FIRST = 4, EPI_FIRST = 8, EPI_WARPS = 8;
 constexpr int THREADS = 32 * (EPI_FIRST + EPI_WARPS);
-constexpr int BOXES = 2;                 // staging boxes per epilogue warp
-constexpr uint32_t BOX_BYTES = 32 * 64;  // 32 rows x 32 bf16
-constexpr uint32_t ACC_STEP = 192;       // second accumulator's first column
-constexpr uint32_t SF_COL = 448;         // scale columns: two slots of 32 (8 for A, 16 for B)
+constexpr uint32_t BOX_BYTES = 32 * 64;  // an epilogue warp's staging box: 32 rows x 32 bf16
+constexpr uint32_t SF_COL = 256;         // first scale column
 constexpr uint32_t TMEM_COLS = 512;
+constexpr size_t kSmemLimit = 232448;
+// Registers: launched at 128 per thread (512 threads), then 56 for the producer and
+// scale warpgroups and 200 for the two of the epilogue: 256 * 56 + 256 * 200 = 512 * 128.
+constexpr int LAUNCH_REGS = 128, REG_LOW = 56, REG_EPI = 200;
+static_assert(256 * REG_LOW + 256 * REG_EPI <= THREADS * LAUNCH_REGS, "the split must fit the launch allocation");
 
 struct Params {
   const int32_t* offsets;  // [segs] inclusive row ends
@@ -337,8 +346,11 @@ struct Params {
   int64_t S;
   int K, N;                // reduction length; output columns (I or H)
   int n_tiles;
+  int n_run;               // column tiles a unit walks over
   int w_blocks;            // row tiles of one expert's scales
   int has_ext;
+  int a_bufs, b_stages;    // ring sizes
+  int resident;            // 1: a row tile's A stays for the unit's whole run
   __nv_bfloat16* out;      // h [S, I] or y [S, H]; GATEUP: may be null when hq is wanted alone
   __nv_bfloat16* gate_up;  // GATEUP: optional [S, 2I]
   uint8_t* hq;             // GATEUP: optional packed h [S, I/2] ...
@@ -348,22 +360,32 @@ struct Params {
 };
 
 struct alignas(16) Smem {
-  uint64_t full[STAGES];
-  uint64_t empty[STAGES];
-  uint64_t tfull[2];
-  uint64_t tover;
+  uint64_t a_full[A_BUFS];      // leader: both CTAs' bytes
+  uint64_t a_empty[A_BUFS];
+  uint64_t b_full[B_STAGES];    // leader: both CTAs' bytes and scale warps
+  uint64_t b_empty[B_STAGES];
+  uint64_t sf_full[B_STAGES];   // this CTA's scale bytes
+  uint64_t tfull;
+  uint64_t tempty;              // leader: both CTAs' epilogue warps
   uint32_t tmem_base;
   int abort_flag;
-  int warp_sum[32];
-  int row_start[kMaxSegs + 1];
-  int tile_prefix[kMaxSegs + 1];
-  int blk_prefix[kMaxSegs + 1];
+  int segs;                     // followed by row_start, tile_prefix, blk_prefix [segs + 1]
+  int pad;
 };
-
-constexpr size_t smem_bytes() {
-  return 1024 + (size_t)STAGES * STAGE_BYTES + (size_t)EPI_WARPS * BOXES * BOX_BYTES + sizeof(Smem);
+struct Table {  // the segment table behind Smem
+  int* row_start;
+  int* tile_prefix;  // 256-row tiles before a segment
+  int* blk_prefix;   // 128-row scale blocks before it
+};
+__host__ __device__ inline size_t table_bytes(int segs) { return ((size_t)3 * (segs + 1) * sizeof(int) + 15) / 16 * 16; }
+__device__ __forceinline__ Table table_of(Smem& sm, int segs) {
+  int* t = reinterpret_cast<int*>(&sm + 1);
+  return Table{t, t + segs + 1, t + 2 * (segs + 1)};
 }
-static_assert(smem_bytes() <= 232448, "shared memory budget exceeded");
+inline size_t smem_bytes(int a_bufs, int b_stages, int segs) {
+  return 1024 + (size_t)a_bufs * A_BYTES + (size_t)b_stages * (B_BYTES + SF_BYTES) +
+         EPI_WARPS * BOX_BYTES + sizeof(Smem) + table_bytes(segs);
+}
 
 // Instruction descriptor of kind::mxf4: E2M1 operands, both K-major, UE8M0
 // scales; sf_id (0 or 2) picks the two scale bytes of the K = 64 step.
@@ -372,46 +394,77 @@ __device__ __forceinline__ constexpr uint32_t idesc_mxf4(int M, int N, uint32_t 
          (sf_id << 29);
 }
 
-__device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+// Shared-memory descriptors are built from their low words (address / 16, the only
+// part that changes) to keep the issuing thread's instructions few: it shares its
+// scheduler with epilogue warps, and every instruction between two MMAs is a gap.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row groups 1 KB apart, sm_100, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFF) >> 4) | (1u << 16); }
+
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa,
                                                uint32_t sfb, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %7};\n\t"
+      "mov.b64 db, {%2, %7};\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(DESC_HI)
       : "memory");
 }
 
-// One 512-byte scale tile (32 rows of 16 bytes) into 4 TMEM columns, copied to
-// all four lane quarters, in both CTAs of the pair.
-__device__ __forceinline__ void scale_copy_pair(uint32_t tmem, uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(128 >> 4) << 32;  // 8-row groups 128 bytes apart
-  d |= (uint64_t)1 << 46;           // sm_100 descriptor, no swizzle
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+// Eight columns of this warp's 32 TMEM lanes.
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, uint4 a, uint4 b) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(a.x),
+               "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
 }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// g / (1 + 2^(-g log2 e)) in four instructions: the flushing approximations (2^-22
+// relative) drop the subnormal handling of expf and a division, which doubled the
+// gate/up epilogue's instructions.  g below -88 gives -0.
+__device__ __forceinline__ float silu(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
+}
+
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Segment table shared by every role: first rows, and exclusive prefixes of the
 // 256-row tiles and of the 128-row scale blocks.  All threads take part.
-__device__ __forceinline__ void build_segments(Smem& sm, const int32_t* offsets, int segs, int64_t S, int site) {
+__device__ __forceinline__ void build_segments(const Table& tb, const int32_t* offsets, int segs, int64_t S, int site) {
   for (int g = threadIdx.x; g < segs; g += THREADS) {
     int begin;
     const int rows = segment_rows(offsets, g, S, begin, site);
-    sm.row_start[g] = begin;
-    sm.blk_prefix[g] = rows;  // until the scan below
+    tb.row_start[g] = begin;
+    tb.blk_prefix[g] = rows;  // until the scan below
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int tiles = 0, blocks = 0, end = 0;
+    int tiles = 0, blocks = 0;
     for (int g0 = 0; g0 < segs; g0 += 32) {
       const int g = g0 + lane;
-      const int rows = g < segs ? sm.blk_prefix[g] : 0;
+      const int rows = g < segs ? tb.blk_prefix[g] : 0;
       const int t = (rows + TILE_M - 1) / TILE_M, b = (rows + BM - 1) / BM;
       int ti = t, bi = b;
 #pragma unroll
@@ -420,31 +473,41 @@ __device__ __forceinline__ void build_segments(Smem& sm, const int32_t* offsets,
         if (lane >= o) ti += tv, bi += bv;
       }
       if (g < segs) {
-        sm.tile_prefix[g] = tiles + ti - t;
-        sm.blk_prefix[g] = blocks + bi - b;
-        end = sm.row_start[g] + rows;
-        if (g == segs - 1) sm.row_start[segs] = end;
+        tb.tile_prefix[g] = tiles + ti - t;
+        tb.blk_prefix[g] = blocks + bi - b;
+        if (g == segs - 1) tb.row_start[segs] = tb.row_start[g] + rows;
       }
       tiles += __shfl_sync(0xffffffffu, ti, 31);
       blocks += __shfl_sync(0xffffffffu, bi, 31);
     }
-    if (lane == 0) sm.tile_prefix[segs] = tiles, sm.blk_prefix[segs] = blocks;
+    if (lane == 0) tb.tile_prefix[segs] = tiles, tb.blk_prefix[segs] = blocks;
   }
 }
 
-struct Tile {
-  int seg, m, n;
+// Unit u: a row tile and a run of column tiles.  Runs are the outer index, so
+// that the pairs at work together share experts' B tiles in L2.
+struct Unit {
+  int seg, m, n0, n1;
 };
-__device__ __forceinline__ Tile decode_tile(const Smem& sm, int t, int segs, int n_tiles) {
-  const int mt = t / n_tiles;
-  int lo = 0, hi = segs;
+__device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Params& p) {
+  const int tiles = tb.tile_prefix[p.segs];
+  const int run = u / tiles, mt = u - run * tiles;
+  int lo = 0, hi = p.segs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (sm.tile_prefix[mid] <= mt) lo = mid;
+    if (tb.tile_prefix[mid] <= mt) lo = mid;
     else hi = mid;
   }
-  return Tile{lo, mt - sm.tile_prefix[lo], t - mt * n_tiles};
+  return Unit{lo, mt - tb.tile_prefix[lo], run * p.n_run, min(p.n_tiles, (run + 1) * p.n_run)};
 }
+
+struct Ring {  // position in a ring of buffers
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++i == size) i = 0, phase ^= 1;
+  }
+};
 
 template <int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -453,33 +516,35 @@ __global__ void __launch_bounds__(THREADS, 1)
                    const __grid_constant__ CUtensorMap tmap_sb0, const __grid_constant__ CUtensorMap tmap_sb1,
                    const __grid_constant__ CUtensorMap tmap_xa, const __grid_constant__ CUtensorMap tmap_xb,
                    const __grid_constant__ CUtensorMap tmap_o0, const __grid_constant__ CUtensorMap tmap_o1,
-                   const __grid_constant__ CUtensorMap tmap_o2, const Params p) {
+                   const __grid_constant__ CUtensorMap tmap_o2, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = base;
-  uint8_t* sB = sA + STAGES * A_BYTES;
-  uint8_t* sBox = sB + STAGES * B_BYTES;  // 1024-byte aligned like the operands
-  uint8_t* sSA = sBox + EPI_WARPS * BOXES * BOX_BYTES;
-  uint8_t* sSB = sSA + STAGES * SFA_BYTES;
-  Smem& sm = *reinterpret_cast<Smem*>(sSB + STAGES * SFB_BYTES);
+  uint8_t* sB = sA + p.a_bufs * A_BYTES;
+  uint8_t* sBox = sB + p.b_stages * B_BYTES;
+  uint8_t* sSF = sBox + EPI_WARPS * BOX_BYTES;  // per stage: A tiles, then B's two halves
+  Smem& sm = *reinterpret_cast<Smem*>(sSF + p.b_stages * SF_BYTES);
+  const Table tb = table_of(sm, p.segs);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int unit = (int)(blockIdx.x >> 1), num_units = (int)(gridDim.x >> 1);
-  const uint32_t full_leader0 = mapa_shared(smem_u32(&sm.full[0]), 0);
-  const uint32_t tover_leader = mapa_shared(smem_u32(&sm.tover), 0);
+  const int first_unit = (int)(blockIdx.x >> 1), num_pairs = (int)(gridDim.x >> 1);
 
-  build_segments(sm, p.offsets, p.segs, p.S, 710 + MODE);
+  build_segments(tb, p.offsets, p.segs, p.S, 710 + MODE);
   if (warp == 1) {
     if (lane == 0) {
-      for (int s = 0; s < STAGES; ++s) {
-        mbar_init(&sm.full[s], 1);
-        mbar_init(&sm.empty[s], 1);
+      for (int i = 0; i < A_BUFS; ++i) {
+        mbar_init(&sm.a_full[i], 1);
+        mbar_init(&sm.a_empty[i], 1);
       }
-      mbar_init(&sm.tfull[0], 1);
-      mbar_init(&sm.tfull[1], 1);
-      mbar_init(&sm.tover, 2 * EPI_WARPS);
+      for (int i = 0; i < B_STAGES; ++i) {
+        mbar_init(&sm.b_full[i], 1 + 2 * 4);  // the leader's producer, and the scale warps of both CTAs
+        mbar_init(&sm.b_empty[i], 1);
+        mbar_init(&sm.sf_full[i], 1);
+      }
+      mbar_init(&sm.tfull, 1);
+      mbar_init(&sm.tempty, 2 * EPI_WARPS);
       sm.abort_flag = 0;
       fence_mbar_init();
     }
@@ -503,242 +568,298 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
 
   const uint32_t tmem = sm.tmem_base;
-  const int total_tiles = sm.tile_prefix[p.segs] * p.n_tiles;
+  if (tmem != 0 && threadIdx.x == 0) device_fail(MIRAI_ERR_DEVICE_BOUNDS, 715);  // cannot be: see the MMA issuer
+  const int num_units = tb.tile_prefix[p.segs] * ((p.n_tiles + p.n_run - 1) / p.n_run);
   const int num_kb = (p.K + BKE - 1) / BKE;
   const int total_kb = num_kb + p.has_ext;
   volatile int* abort_flag = &sm.abort_flag;
 
-  if (warp == 0 && lane == 0) {
-    // ======================= TMA producer =======================
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int t = unit; t < total_tiles && !*abort_flag; t += num_units) {
-      const Tile tile = decode_tile(sm, t, p.segs, p.n_tiles);
-      const int e = tile.seg % p.experts;
-      const int row = sm.row_start[tile.seg] + tile.m * TILE_M + (int)rank * BM;
-      const int ablk = sm.blk_prefix[tile.seg] + tile.m * 2 + (int)rank;
-      // B rows of this CTA, and the row tiles of both halves' scales
-      const CUtensorMap* mb = MODE == GATEUP && rank ? &tmap_b1 : &tmap_b0;
-      const int brow = e * p.N + (MODE == GATEUP ? tile.n * BM : tile.n * TN + (int)rank * BM);
-      const int bblk = e * p.w_blocks + (MODE == GATEUP ? tile.n : 2 * tile.n);
-      for (int kb = 0; kb < total_kb; ++kb) {
-        if (!mbar_wait(&sm.empty[stage], phase ^ 1, 70)) {
+  if (warp < SF_FIRST) {
+    regs_dec<REG_LOW>();
+    if (warp == 0 && lane == 0) {
+      // ======================= TMA producer =======================
+      const uint32_t a_full0 = mapa_shared(smem_u32(&sm.a_full[0]), 0), b_full0 = mapa_shared(smem_u32(&sm.b_full[0]), 0);
+      Ring ra, rb;
+      for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
+        const Unit un = decode_unit(tb, u, p);
+        const int e = un.seg % p.experts;
+        const int row = tb.row_start[un.seg] + un.m * TILE_M + (int)rank * BM;
+        const CUtensorMap* mb = MODE == GATEUP && rank ? &tmap_b1 : &tmap_b0;
+        for (int n = un.n0; n < un.n1 && !*abort_flag; ++n) {
+          const int brow = e * p.N + (MODE == GATEUP ? n * BM : n * TN + (int)rank * BM);  // B rows of this CTA
+          for (int kb = 0; kb < total_kb; ++kb) {
+            const bool ext = kb == num_kb;
+            if (n == un.n0 || !p.resident) {
+              if (!mbar_wait(&sm.a_empty[ra.i], ra.phase ^ 1, 70)) {
+                *abort_flag = 1;
+                break;
+              }
+              // the leader's own barrier carries the bytes of both CTAs
+              if (leader) mbar_arrive_expect_tx(&sm.a_full[ra.i], 2 * A_BYTES);
+              tma_load_2d_pair(sA + ra.i * A_BYTES, ext ? &tmap_xa : &tmap_a, ext ? 0 : kb * 128, row, a_full0 + 8u * ra.i);
+              ra.next(p.a_bufs);
+            }
+            if (!mbar_wait(&sm.b_empty[rb.i], rb.phase ^ 1, 71)) {
+              *abort_flag = 1;
+              break;
+            }
+            if (leader) mbar_arrive_expect_tx(&sm.b_full[rb.i], 2 * B_BYTES);
+            tma_load_2d_pair(sB + rb.i * B_BYTES, ext ? &tmap_xb : mb, ext ? 0 : kb * 128, brow, b_full0 + 8u * rb.i);
+            rb.next(p.b_stages);
+          }
+        }
+      }
+      // no commit of the leader may reach this CTA after it has exited
+      for (int i = 0; i < p.b_stages; ++i) {
+        if (!mbar_wait(&sm.b_empty[rb.i], rb.phase ^ 1, 72)) break;
+        rb.next(p.b_stages);
+      }
+      for (int i = 0; i < p.a_bufs; ++i) {
+        if (!mbar_wait(&sm.a_empty[ra.i], ra.phase ^ 1, 73)) break;
+        ra.next(p.a_bufs);
+      }
+    } else if (warp == 2 && lane == 0) {
+      // ======================= TMA producer of the scales =======================
+      Ring rb;
+      for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
+        const Unit un = decode_unit(tb, u, p);
+        const int e = un.seg % p.experts;
+        const int ablk = tb.blk_prefix[un.seg] + un.m * 2 + (int)rank;
+        for (int n = un.n0; n < un.n1 && !*abort_flag; ++n) {
+          // row tiles of both column halves
+          const int bblk = e * p.w_blocks + (MODE == GATEUP ? n : 2 * n);
+          for (int kb = 0; kb < total_kb; ++kb) {
+            if (!mbar_wait(&sm.b_empty[rb.i], rb.phase ^ 1, 79)) {
+              *abort_flag = 1;
+              break;
+            }
+            uint64_t* sf = &sm.sf_full[rb.i];
+            if (kb == num_kb) {
+              mbar_arrive(sf);  // the rank block has no scales
+            } else {
+              uint8_t* dst = sSF + rb.i * SF_BYTES;
+              mbar_arrive_expect_tx(sf, SF_BYTES);
+              tma_load_2d(dst, &tmap_sa, kb * 256, ablk, sf);
+              tma_load_2d(dst + 1024, &tmap_sb0, kb * 256, bblk, sf);
+              tma_load_2d(dst + 2048, MODE == GATEUP ? &tmap_sb1 : &tmap_sb0, kb * 256, MODE == GATEUP ? bblk : bblk + 1, sf);
+            }
+            rb.next(p.b_stages);
+          }
+        }
+      }
+    } else if (warp == 1 && leader) {
+      // ======================= MMA issuer =======================
+      // The whole warp runs the loop, so that its operands stay in uniform
+      // registers; one elected lane issues.
+      const bool issue = elect_one();
+      constexpr uint32_t id_ext = make_idesc_bf16(TILE_M, TN);
+      constexpr uint32_t id0 = idesc_mxf4(TILE_M, TN, 0), id2 = idesc_mxf4(TILE_M, TN, 2);
+      const uint32_t a_lo0 = desc_lo(smem_u32(sA)), b_lo0 = desc_lo(smem_u32(sB));
+      const int last_steps = (p.K - (num_kb - 1) * BKE + 63) / 64;  // K = 64 steps of the last k-block
+      Ring ra, rb;
+      constexpr uint32_t acc = 0;  // all 512 columns are this CTA's: they start at 0 (checked above)
+      uint32_t tiles = 0;
+      bool ok = true;
+      for (int u = first_unit; u < num_units && ok && !*abort_flag; u += num_pairs) {
+        const Unit un = decode_unit(tb, u, p);
+        const Ring ra0 = ra;
+        for (int n = un.n0; n < un.n1 && ok; ++n, ++tiles) {
+          if (p.resident) ra = ra0;
+          const bool first = n == un.n0 || !p.resident, last = n + 1 == un.n1 || !p.resident;
+          if (tiles > 0 && !mbar_wait(&sm.tempty, (tiles - 1) & 1, 74)) ok = false;
+          for (int kb = 0; kb < total_kb && ok; ++kb) {
+            if ((first && !mbar_wait(&sm.a_full[ra.i], ra.phase, 75)) || !mbar_wait(&sm.b_full[rb.i], rb.phase, 76)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a = a_lo0 + ra.i * (A_BYTES >> 4), b = b_lo0 + rb.i * (B_BYTES >> 4);
+            const uint32_t sf = SF_COL + rb.i * 32;
+            if (issue) {
+              if (kb < num_kb - 1 || (kb < num_kb && last_steps == 4)) {
+                umma_mxf4_pair(acc, a, b, id0, sf, sf + 8, kb != 0);
+                umma_mxf4_pair(acc, a + 2, b + 2, id2, sf, sf + 8, 1);
+                umma_mxf4_pair(acc, a + 4, b + 4, id0, sf + 4, sf + 16, 1);
+                umma_mxf4_pair(acc, a + 6, b + 6, id2, sf + 4, sf + 16, 1);
+              } else if (kb < num_kb) {
+                umma_mxf4_pair(acc, a, b, id0, sf, sf + 8, kb != 0);
+                if (last_steps > 1) umma_mxf4_pair(acc, a + 2, b + 2, id2, sf, sf + 8, 1);
+                if (last_steps > 2) umma_mxf4_pair(acc, a + 4, b + 4, id0, sf + 4, sf + 16, 1);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  umma_bf16_pair(acc, ((uint64_t)DESC_HI << 32) | (a + 2 * k), ((uint64_t)DESC_HI << 32) | (b + 2 * k),
+                                 id_ext, 1u);
+              }
+              umma_commit_pair(&sm.b_empty[rb.i], 0x3);
+              if (last) umma_commit_pair(&sm.a_empty[ra.i], 0x3);
+            }
+            __syncwarp();
+            rb.next(p.b_stages);
+            ra.next(p.a_bufs);
+          }
+          if (ok && issue) umma_commit_pair(&sm.tfull, 0x3);
+          __syncwarp();
+        }
+      }
+      if (!ok && lane == 0) *abort_flag = 1;
+    }
+  } else if (warp < EPI_FIRST) {
+    // ======================= scales: shared memory -> TMEM =======================
+    // A scale tile is 32 lanes x 16 bytes: lane l holds rows l, l + 32, l + 64, l + 96,
+    // one column each; every lane quarter gets a copy, its own warp's.
+    regs_dec<REG_LOW>();
+    const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t b_full0 = mapa_shared(smem_u32(&sm.b_full[0]), 0);
+    Ring rb;
+    for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
+      const Unit un = decode_unit(tb, u, p);
+      const int blocks = (un.n1 - un.n0) * total_kb;
+      int kb = 0;
+      for (int i = 0; i < blocks; ++i) {
+        if (!mbar_wait(&sm.sf_full[rb.i], rb.phase, 77)) {
           *abort_flag = 1;
           break;
         }
-        const uint32_t full = full_leader0 + 8u * stage;
-        const bool ext = kb == num_kb;
-        // the leader's own barrier carries the bytes of both CTAs
-        if (leader) mbar_arrive_expect_tx(&sm.full[stage], 2 * (ext ? A_BYTES + B_BYTES : STAGE_BYTES));
-        if (ext) {
-          tma_load_2d_pair(sA + stage * A_BYTES, &tmap_xa, 0, row, full);
-          tma_load_2d_pair(sB + stage * B_BYTES, &tmap_xb, 0, brow, full);
-        } else {
-          tma_load_2d_pair(sA + stage * A_BYTES, &tmap_a, kb * 128, row, full);
-          tma_load_2d_pair(sB + stage * B_BYTES, mb, kb * 128, brow, full);
-          tma_load_2d_pair(sSA + stage * SFA_BYTES, &tmap_sa, kb * 256, ablk, full);
-          tma_load_2d_pair(sSB + stage * SFB_BYTES, &tmap_sb0, kb * 256, bblk, full);
-          tma_load_2d_pair(sSB + stage * SFB_BYTES + 1024, MODE == GATEUP ? &tmap_sb1 : &tmap_sb0, kb * 256,
-                           MODE == GATEUP ? bblk : bblk + 1, full);
+        if (kb != num_kb) {
+          tc_fence_after();  // the MMAs that read this slot have completed (the stage was refilled after them)
+          const uint32_t src = smem_u32(sSF + rb.i * SF_BYTES) + lane * 16u;
+          const uint32_t dst = tmem + SF_COL + rb.i * 32 + quarter;
+          const uint4 a0 = lds128(src), a1 = lds128(src + 512);
+          const uint4 l0 = lds128(src + 1024), l1 = lds128(src + 1536), h0 = lds128(src + 2048), h1 = lds128(src + 2560);
+          tmem_st_x8(dst, a0, a1);
+          tmem_st_x8(dst + 8, l0, h0);    // K tile 0: both column halves
+          tmem_st_x8(dst + 16, l1, h1);   // K tile 1
+          tmem_st_wait();
+          tc_fence_before();
         }
-        if (++stage == STAGES) stage = 0, phase ^= 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(b_full0 + 8u * rb.i);
+        rb.next(p.b_stages);
+        kb = kb + 1 == total_kb ? 0 : kb + 1;
       }
     }
-    // no commit of the leader may reach this CTA after it has exited
-    for (int i = 0; i < STAGES; ++i) {
-      if (!mbar_wait(&sm.empty[stage], phase ^ 1, 71)) break;
-      if (++stage == STAGES) stage = 0, phase ^= 1;
-    }
-  } else if (warp == 1 && lane == 0 && leader) {
-    // ======================= MMA issuer =======================
-    constexpr uint32_t id_ext = make_idesc_bf16(TILE_M, TN);
-    int stage = 0, it = 0;
-    uint32_t phase = 0, slot = 0;
-    for (int t = unit; t < total_tiles && !*abort_flag; t += num_units, ++it) {
-      // the epilogue has read the columns this accumulator shares with the
-      // previous tile's (and with it all of the tile before that one)
-      if (it > 0 && !mbar_wait(&sm.tover, (it - 1) & 1, 72)) {
-        *abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t d = tmem + (it & 1) * ACC_STEP;
+  } else {
+    // ======================= epilogue =======================
+    regs_inc<REG_EPI>();
+    const int q = warp & 3;                  // TMEM lane quarter
+    const int part = (warp - EPI_FIRST) / 4;  // its half of the columns
+    const uint32_t tempty_leader = mapa_shared(smem_u32(&sm.tempty), 0);
+    const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16);
+    uint8_t* box = sBox + (warp - EPI_FIRST) * BOX_BYTES;
+    const uint32_t box_row = smem_u32(box) + (uint32_t)lane * 64u;
+    const uint32_t box_sw = (uint32_t)(lane >> 1) & 3u;  // 64-byte swizzle: 16-byte chunk ^= row bits 1..2
+    uint32_t tiles = 0;
+    for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
+      const Unit un = decode_unit(tb, u, p);
+      const int local = un.m * TILE_M + (int)rank * BM + q * 32 + lane;
+      const int64_t row = (int64_t)tb.row_start[un.seg] + local;
+      const bool valid = row < tb.row_start[un.seg + 1];
+      const bool boxed = __all_sync(0xffffffffu, valid);  // all 32 rows are the segment's
+      const int row0 = (int)(row - lane);
+      // 32 rows x 32 columns: through the staging box and one TMA store, or row by row.  (A lane
+      // storing its own row straight to global memory touches 32 lines per store: 33 us more on the
+      // 32768-token layer's gate/up.)
+      auto store = [&](const CUtensorMap* map, __nv_bfloat16* dst, int col, const uint32_t* w) {
+        if (boxed) {
+          if (lane == 0) bulk_wait_group_read<0>();  // the box's previous store has read it
+          __syncwarp();
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            sts128(box_row + (((uint32_t)v ^ box_sw) << 4), w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map, box, col, row0);
+            bulk_commit_group();
+          }
+        } else if (valid) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            reinterpret_cast<uint4*>(dst)[v] = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
+        }
+      };
       bool ok = true;
-      for (int kb = 0; kb < total_kb; ++kb) {
-        if (!mbar_wait(&sm.full[stage], phase, 73)) {
+      for (int n = un.n0; n < un.n1 && ok; ++n, ++tiles) {
+        if (!mbar_wait(&sm.tfull, tiles & 1, 78)) {
+          *abort_flag = 1;
           ok = false;
           break;
         }
+        __syncwarp();
         tc_fence_after();
-        const uint32_t a = smem_u32(sA + stage * A_BYTES), b = smem_u32(sB + stage * B_BYTES);
-        if (kb == num_kb) {
+        uint32_t v[4][32];
+        // GATEUP: channels of chunks 2 part, 2 part + 1: gate in v[0], v[1], up in v[2], v[3].
+        // DOWN: column chunks 4 part .. 4 part + 3.
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_pair(d, make_sdesc_sw128(a + k * 32, 16, 1024), make_sdesc_sw128(b + k * 32, 16, 1024), id_ext, 1u);
-        } else {
-          const uint32_t sf = tmem + SF_COL + slot * 32;
-          slot ^= 1;
-          const uint32_t sa = smem_u32(sSA + stage * SFA_BYTES), sb = smem_u32(sSB + stage * SFB_BYTES);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            scale_copy_pair(sf + 4 * w, sa + 512 * w);
-            scale_copy_pair(sf + 8 + 8 * w, sb + 512 * w);
-            scale_copy_pair(sf + 8 + 8 * w + 4, sb + 1024 + 512 * w);
-          }
-          const int steps = min(4, (p.K - kb * BKE + 63) / 64);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k < steps)
-              umma_mxf4_pair(d, make_sdesc_sw128(a + k * 32, 16, 1024), make_sdesc_sw128(b + k * 32, 16, 1024),
-                             idesc_mxf4(TILE_M, TN, (k & 1) * 2), sf + 4 * (k >> 1), sf + 8 + 8 * (k >> 1),
-                             (kb | k) != 0 ? 1u : 0u);
-          }
-        }
-        umma_commit_pair(&sm.empty[stage], 0x3);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
-      }
-      if (!ok) {
-        *abort_flag = 1;
-        break;
-      }
-      umma_commit_pair(&sm.tfull[it & 1], 0x3);
-    }
-  } else if (warp >= EPI_FIRST) {
-    // ======================= epilogue =======================
-    const int q = warp & 3;                     // TMEM lane quarter
-    const int part = (warp - EPI_FIRST) / 4;    // which half of the 32-column chunks
-    uint8_t* my_boxes = sBox + (warp - EPI_FIRST) * BOXES * BOX_BYTES;
-    int box_i = 0;
-    auto stage_store = [&](const CUtensorMap* map, int col, int64_t row0, const uint32_t (&w)[16]) {
-      uint8_t* box = my_boxes + box_i * BOX_BYTES;
-      if (lane == 0) bulk_wait_group_read<BOXES - 1>();
-      __syncwarp();
-      const uint32_t addr = smem_u32(box) + (uint32_t)lane * 64u;
-      const uint32_t sw = (uint32_t)(lane >> 1) & 3u;  // 64-byte swizzle
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        sts128(addr + (((uint32_t)v ^ sw) << 4), w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(map, box, col, (int)row0);
-        bulk_commit_group();
-      }
-      box_i = box_i + 1 == BOXES ? 0 : box_i + 1;
-    };
-    auto row_store = [&](__nv_bfloat16* dst, const uint32_t (&w)[16]) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        reinterpret_cast<uint4*>(dst)[v] = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
-    };
-    int it = 0;
-    for (int t = unit; t < total_tiles && !*abort_flag; t += num_units, ++it) {
-      const Tile tile = decode_tile(sm, t, p.segs, p.n_tiles);
-      const int begin = sm.row_start[tile.seg];
-      // a segment ends where its tiles say (bad offsets may leave gaps between segments)
-      const int end = sm.row_start[tile.seg + 1];
-      const int local = tile.m * TILE_M + (int)rank * BM + q * 32 + lane;
-      const bool valid = begin + local < end;
-      const int64_t row = (int64_t)begin + local;
-      const bool boxed = __all_sync(0xffffffffu, valid);
-      const int64_t row0 = __shfl_sync(0xffffffffu, row, 0);
-      if (!mbar_wait(&sm.tfull[it & 1], (it >> 1) & 1, 74)) {
-        *abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t acc = tmem + (it & 1) * ACC_STEP + ((uint32_t)(q * 32) << 16);
-      auto release = [&]() {  // the shared columns have been read
+        for (int i = 0; i < 4; ++i)
+          tmem_ld_32x32b_x32(acc + (MODE == GATEUP ? (i / 2) * BM + part * 64 + (i % 2) * 32 : part * BM + i * 32), v[i]);
+        tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tover_leader);
-      };
-      if constexpr (MODE == GATEUP) {
-        // shared columns: up channels 64..127 of the first accumulator, gate
-        // channels 0..63 of the second
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          const int c = part + (((it & 1) ^ i) ? 0 : 2);
-          uint32_t g[32], u[32];
-          tmem_ld_32x32b_x32(acc + c * 32, g);
-          tmem_ld_32x32b_x32(acc + BM + c * 32, u);
-          tmem_ld_wait();
-          if (i == 0) release();
-          const int col = tile.n * BM + c * 32;
-          if (col >= p.N) continue;  // warp-uniform
-          uint32_t w[16];
-          if (p.gate_up) {
-            const int64_t ld2 = 2 * (int64_t)p.N;
+        if (lane == 0) mbar_arrive_cluster(tempty_leader);
+        if constexpr (MODE == GATEUP) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1]));
-            if (boxed) stage_store(&tmap_o1, col, row0, w);
-            else if (valid) row_store(p.gate_up + row * ld2 + col, w);
+          for (int i = 0; i < 2; ++i) {
+            const int c = 2 * part + i;
+            const int col = n * BM + c * 32;
+            if (col >= p.N) break;  // warp-uniform
+            uint32_t w[16];
+            if (p.gate_up) {
+              __nv_bfloat16* dst = p.gate_up + row * 2 * (int64_t)p.N + col;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
-            if (boxed) stage_store(&tmap_o2, col, row0, w);
-            else if (valid) row_store(p.gate_up + row * ld2 + p.N + col, w);
-          }
+              for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1]));
+              store(&tmap_o1, dst, col, w);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float h[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const float gv = __uint_as_float(g[2 * j + s]);
-              h[s] = __fdividef(gv, 1.f + __expf(-gv)) * __uint_as_float(u[2 * j + s]);
+              for (int j = 0; j < 16; ++j)
+                w[j] = pack_bf16x2(__uint_as_float(v[i + 2][2 * j]), __uint_as_float(v[i + 2][2 * j + 1]));
+              store(&tmap_o2, dst + p.N, col, w);
             }
-            w[j] = pack_bf16x2(h[0], h[1]);
-          }
-          if (p.out) {
-            if (boxed) stage_store(&tmap_o0, col, row0, w);
-            else if (valid) row_store(p.out + row * p.N + col, w);
-          }
-          if (p.hq && valid) {
-            // this lane's 32 channels are one block of the quantised h
-            uint32_t m = 0;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              m = max(m, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
-            const uint32_t byte = scale_byte(m);
-            const float inv = inv_scale(byte == 255u ? 254u : byte);
-            uint32_t codes[4];
+              w[j] = pack_bf16x2(silu(__uint_as_float(v[i][2 * j])) * __uint_as_float(v[i + 2][2 * j]),
+                                 silu(__uint_as_float(v[i][2 * j + 1])) * __uint_as_float(v[i + 2][2 * j + 1]));
+            if (p.out) store(&tmap_o0, p.out + row * p.N + col, col, w);
+            if (p.hq && valid) {
+              // this lane's 32 channels are one block of the quantised h
+              uint32_t m = 0;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              float f[8];
+              for (int j = 0; j < 16; ++j) m = max(m, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
+              const uint32_t byte = scale_byte(m);
+              const float inv = inv_scale(byte == 255u ? 254u : byte);
+              uint32_t codes[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) f[2 * j] = bf16_lo(w[4 * v + j]) * inv, f[2 * j + 1] = bf16_hi(w[4 * v + j]) * inv;
-              codes[v] = byte == 255u ? 0u : e2m1x8(f);
-            }
-            *reinterpret_cast<uint4*>(p.hq + (row * p.N + col) / 2) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-            const int64_t blk = sm.blk_prefix[tile.seg] + tile.m * 2 + (int)rank;
-            if (blk < p.h_blocks) {
-              uint8_t* word = p.hscale + (blk * p.h_kt + tile.n) * 512 + lane * 16 + q * 4;
-              word[c] = (uint8_t)byte;
-              if (col + 32 == p.N)  // blocks past the row's end are zero bytes
-                for (int z = c + 1; z < 4; ++z) word[z] = 0;
+              for (int x = 0; x < 4; ++x) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  f[2 * j] = bf16_lo(w[4 * x + j]) * inv, f[2 * j + 1] = bf16_hi(w[4 * x + j]) * inv;
+                codes[x] = byte == 255u ? 0u : e2m1x8(f);
+              }
+              *reinterpret_cast<uint4*>(p.hq + (row * p.N + col) / 2) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+              const int64_t blk = tb.blk_prefix[un.seg] + un.m * 2 + (int)rank;
+              if (blk < p.h_blocks) {
+                uint8_t* word = p.hscale + (blk * p.h_kt + n) * 512 + lane * 16 + q * 4;
+                word[c] = (uint8_t)byte;
+                if (col + 32 == p.N)  // blocks past the row's end are zero bytes
+                  for (int z = c + 1; z < 4; ++z) word[z] = 0;
+              }
             }
           }
-        }
-      } else {
-        // shared columns: chunks 6, 7 of the first accumulator, 0, 1 of the second
-        const int first = (it & 1) ? part : 6 + part;
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int c = i == 0 ? first : ((it & 1) ? 2 : 0) + part * 3 + i - 1;
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(acc + c * 32, v);
-          tmem_ld_wait();
-          if (i == 0) release();
-          const int col = tile.n * TN + c * 32;
-          if (col >= p.N) continue;  // warp-uniform
-          uint32_t w[16];
+        } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-          if (boxed) stage_store(&tmap_o0, col, row0, w);
-          else if (valid) row_store(p.out + row * p.N + col, w);
+          for (int i = 0; i < 4; ++i) {
+            const int col = n * TN + part * BM + i * 32;
+            if (col >= p.N) break;  // warp-uniform
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1]));
+            store(&tmap_o0, p.out + row * p.N + col, col, w);
+          }
         }
       }
     }
-    if (lane == 0) bulk_wait_group_all();
+    if (lane == 0) bulk_wait_group_all();  // the stores have read the box before the CTA exits
     __syncwarp();
   }
 
@@ -772,7 +893,8 @@ static int out_map(CUtensorMap& m, void* out, int64_t rows, int N, int64_t ld) {
                       32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// CTA pairs of the kernel that fit the current device at once (per device; 0 = an error was set).
+// CTA pairs of the kernel that are resident at once on the current device (0 = an
+// error was set).  Shared memory allows one CTA per SM at every ring size.
 constexpr int kMaxDevices = 64;
 template <int MODE> static int resident_pairs(const char* name) {
   static std::atomic<int> cached[kMaxDevices];
@@ -784,14 +906,21 @@ template <int MODE> static int resident_pairs(const char* name) {
   int n = cached[dev].load(std::memory_order_acquire);
   if (n > 0) return n;
   auto kern = product_kernel<MODE>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes());
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kern);
   if (e != cudaSuccess) {
-    set_error(MIRAI_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", name, cudaGetErrorString(e));
+    set_error(MIRAI_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    return 0;
+  }
+  if (fa.numRegs < LAUNCH_REGS) {
+    set_error(MIRAI_ERR_UNSUPPORTED, "%s compiled with %d registers per thread; the register split needs %d", name,
+              fa.numRegs, LAUNCH_REGS);
     return 0;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(THREADS, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes();
+  cfg.dynamicSmemBytes = kSmemLimit;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -852,7 +981,7 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   p.hscale = hscale;
   p.h_blocks = max_blocks(S, segs);
   p.h_kt = (int)ceil_div(N, 128);
-  CUtensorMap ta, tsa, tb0, tb1, tsb0, tsb1, txa, txb, to0, to1, to2;
+  CUtensorMap ta, tsa, tb0, tb1, tsb0, tsb1, txa, txb;
   int rc = code_map(ta, a.packed, S, K);
   if (!rc) rc = scale_map(tsa, a.scale, p.h_blocks, kt);
   if (!rc) rc = code_map(tb0, w0->packed, (int64_t)experts * N, K);
@@ -869,24 +998,42 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
       rc = make_tmap_2d(&txb, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rank_b, 64, (uint64_t)experts * N, 128, 64, BM,
                         CU_TENSOR_MAP_SWIZZLE_128B);
   }
-  if (!rc) rc = out ? out_map(to0, out, S, N, N) : (to0 = ta, MIRAI_OK);
-  to1 = to2 = to0;
+  CUtensorMap to0 = ta, to1 = ta, to2 = ta;
+  if (!rc && out) rc = out_map(to0, out, S, N, N);
   if (!rc && gate_up) {
     rc = out_map(to1, gate_up, S, N, 2 * (int64_t)N);
     if (!rc) rc = out_map(to2, static_cast<__nv_bfloat16*>(gate_up) + N, S, N, 2 * (int64_t)N);
   }
   if (rc) return rc;
-  const int pairs = resident_pairs<MODE>(name);
-  if (!pairs) return MIRAI_ERR_CUDA;
+  const int pairs_fit = resident_pairs<MODE>(name);
+  if (!pairs_fit) return MIRAI_ERR_CUDA;
   const int limit = gemm_sm_limit();
-  const int sms = (limit > 0 && limit < sm_count()) ? limit : sm_count();
-  int64_t units = (S / TILE_M + (segs < S ? segs : S)) * p.n_tiles;
+  int pairs = pairs_fit;
+  if (limit > 0 && limit / 2 < pairs) pairs = limit / 2 > 0 ? limit / 2 : 1;
+  const int64_t tiles = S / TILE_M + (segs < S ? segs : S);  // at most; about S / 256 when segments are long
+  // rings: A whole where it fits, the rest for B
+  const int total_kb = (int)ceil_div(K, BKE) + p.has_ext;
+  p.resident = total_kb <= A_BUFS;
+  p.a_bufs = p.resident ? (total_kb < 4 ? 4 : total_kb) : 5;
+  p.b_stages = B_STAGES;
+  while (smem_bytes(p.a_bufs, p.b_stages, p.segs) > kSmemLimit) --p.b_stages;
+  // Column tiles per unit: the run that makes the longest pair's time shortest, a tile counting its
+  // B stream and a unit half a tile more for its A.
+  const int64_t likely = ceil_div(S, TILE_M);
+  p.n_run = 1;
+  if (p.resident) {
+    double best = 0;
+    for (int r = 1; r <= p.n_tiles; ++r) {
+      const double cost = (double)ceil_div(likely * ceil_div(p.n_tiles, r), pairs) * (r + 0.5);
+      if (r == 1 || cost < best) best = cost, p.n_run = r;
+    }
+  }
+  int64_t units = tiles * ceil_div(p.n_tiles, p.n_run);
   if (units > pairs) units = pairs;
-  if (units > sms / 2) units = sms / 2 > 0 ? sms / 2 : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.gridDim = dim3((unsigned)(2 * units), 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes();
+  cfg.dynamicSmemBytes = smem_bytes(p.a_bufs, p.b_stages, p.segs);
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
