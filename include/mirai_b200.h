@@ -566,7 +566,8 @@ size_t mirai_mxfp4_scale_bytes(int32_t num_experts, int64_t out_features, int64_
 size_t mirai_mxfp4_rows_scale_bytes(int64_t num_rows, int32_t num_segments, int32_t width);
 
 /* Quantise a [E, out, in] stack (dtype MIRAI_DTYPE_BF16, _F32 or _F16; in % 32 == 0), and
- * read one back (exact in bf16 and fp32, rounded once to fp16).  Pointers 16-byte aligned. */
+ * read one back (exact in bf16 and fp32, rounded once to fp16).  Codes and scales 16-byte
+ * aligned, weight and out 32-byte aligned. */
 int mirai_mxfp4_quantize(const void* weight, int32_t dtype, int32_t num_experts, int64_t out_features,
                          int64_t in_features, uint8_t* packed, uint8_t* scale, mirai_stream_t stream);
 int mirai_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scale, int32_t num_experts, int64_t out_features,
@@ -576,7 +577,7 @@ int mirai_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scale, int32_t 
  * segment-tiled scales above.  row_index (may be NULL) [num_rows] names the row of x
  * [x_rows, width] each row is read from (the permute of mirai_permute_rows_bf16 in the same
  * pass); offsets [num_segments] int32 inclusive row ends, 1..1024 segments.  Rows past the last
- * segment are not written. */
+ * segment are not written.  x 32-byte aligned. */
 int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_index, const int32_t* offsets,
                               int32_t num_segments, int64_t num_rows, int32_t width, uint8_t* packed, uint8_t* scale,
                               mirai_stream_t stream);

@@ -54,34 +54,59 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   return r;
 }
 
-template <typename T> struct Raw8 { uint4 a; };  // eight 16-bit values
-template <> struct Raw8<float> { uint4 a, b; };
+// Sixteen values of a row as they lie in memory, by 32-byte loads.
+template <typename T> struct Raw16 { uint32_t w[sizeof(T) * 4]; };
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, Raw8<T>& r) {
-  r.a = __ldg(reinterpret_cast<const uint4*>(p));
-  if constexpr (sizeof(T) == 4) r.b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+__device__ __forceinline__ void ldg256(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
 }
-template <typename T> __device__ __forceinline__ void zero8(Raw8<T>& r) {
-  r.a = make_uint4(0, 0, 0, 0);
-  if constexpr (sizeof(T) == 4) r.b = r.a;
+__device__ __forceinline__ void stg256(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
-__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& r, float (&v)[8]) {
-  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+template <typename T> __device__ __forceinline__ void load16(const T* p, Raw16<T>& r) {
+  ldg256(p, r.w);
+  if constexpr (sizeof(T) == 4) ldg256(p + 8, r.w + 8);
+}
+
+// Largest |x| of the sixteen as fp32 bits, by integer maxima (two 16-bit ones per word).
+__device__ __forceinline__ uint32_t amax16(const Raw16<__nv_bfloat16>& r) {
+  uint32_t m = r.w[0] & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, r.w[i] & 0x7fff7fffu);
+  return max(m & 0x7fff0000u, m << 16);
 }
-__device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&v)[8]) {
-  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+__device__ __forceinline__ uint32_t amax16(const Raw16<__half>& r) {
+  uint32_t m = r.w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, r.w[i] & 0x7fff7fffu);
+  const uint32_t top = max(m >> 16, m & 0xffffu);
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+}
+__device__ __forceinline__ uint32_t amax16(const Raw16<float>& r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, r.w[i] & 0x7fffffffu);
+  return m;
+}
+// Eight of them (half h), as floats.
+__device__ __forceinline__ void unpack8(const Raw16<__nv_bfloat16>& r, int h, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(r.w[4 * h + i]), v[2 * i + 1] = bf16_hi(r.w[4 * h + i]);
+}
+__device__ __forceinline__ void unpack8(const Raw16<__half>& r, int h, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[4 * h + i]));
     v[2 * i] = f.x, v[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&v)[8]) {
-  v[0] = __uint_as_float(r.a.x), v[1] = __uint_as_float(r.a.y), v[2] = __uint_as_float(r.a.z);
-  v[3] = __uint_as_float(r.a.w), v[4] = __uint_as_float(r.b.x), v[5] = __uint_as_float(r.b.y);
-  v[6] = __uint_as_float(r.b.z), v[7] = __uint_as_float(r.b.w);
+__device__ __forceinline__ void unpack8(const Raw16<float>& r, int h, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[8 * h + i]);
 }
 
 // Rows [begin, begin + rows) of segment g.  Ends outside [0, S] or below the
@@ -141,11 +166,14 @@ __device__ __forceinline__ RowBlock find_block(const int32_t* __restrict__ offse
 }
 
 // A CTA quantises kStrip rows of one row block, a warp one row at a time: a
-// lane holds 8 elements, four lanes a block (two shuffles for its maximum),
-// a step of the warp 256 elements (512 bytes of bf16 in, 128 bytes of codes
-// out), kAhead steps loaded before the first is used.
+// lane holds 16 elements (one 32-byte load of 16-bit values), two lanes a block (one
+// shuffle for its maximum), a step of the warp 512 elements, kAhead steps
+// loaded before the first is used.  Eight elements per lane and four lanes per block
+// needed half as many instructions again, which bound it.
 constexpr int kStrip = 32;
-constexpr int kAhead = 4;
+constexpr int kAhead = 2;
+constexpr int kStep = 512;
+constexpr int kAheadBack = 4;  // read-back
 
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t x_rows,
@@ -175,36 +203,38 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
       if (!ok && lane == 0) device_fail(MIRAI_ERR_DEVICE_BOUNDS, 701);
     }
     const T* row = x + src * K;
-    for (int k0 = lane * 8; k0 - lane * 8 < K; k0 += 256 * kAhead) {
-      Raw8<T> raw[kAhead];
+    for (int base = 0; base < K; base += kStep * kAhead) {
+      Raw16<T> raw[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        if (ok && k0 + i * 256 < K) load8(row + k0 + i * 256, raw[i]);
-        else zero8(raw[i]);
+        const int k = base + i * kStep + lane * 16;
+        if (ok && k < K) load16(row + k, raw[i]);
+        else raw[i] = Raw16<T>{};
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int k = k0 + i * 256;
-        if (k - lane * 8 >= K) break;  // warp-uniform
-        float v[8];
-        unpack8(raw[i], v);
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        const int k = base + i * kStep + lane * 16;
+        if (base + i * kStep >= K) break;  // warp-uniform
+        uint32_t m = amax16(raw[i]);
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const uint32_t byte = scale_byte(m);
         const float inv = inv_scale(byte == 255u ? 254u : byte);
+        uint32_t codes[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
-        const uint32_t codes = byte == 255u ? 0u : e2m1x8(v);
-        if (k < K) *reinterpret_cast<uint32_t*>(packed + (dst * K + k) / 2) = codes;
+        for (int h = 0; h < 2; ++h) {
+          float v[8];
+          unpack8(raw[i], h, v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= inv;
+          codes[h] = byte == 255u ? 0u : e2m1x8(v);
+        }
+        if (k < K) *reinterpret_cast<uint2*>(packed + (dst * K + k) / 2) = make_uint2(codes[0], codes[1]);
         // four blocks make one word of the row's scales (blocks past K stay zero)
-        uint32_t w = k < K ? byte << (8 * ((lane >> 2) & 3)) : 0u;
+        uint32_t w = k < K ? byte << (8 * ((lane >> 1) & 3)) : 0u;
+        w |= __shfl_xor_sync(0xffffffffu, w, 2);
         w |= __shfl_xor_sync(0xffffffffu, w, 4);
-        w |= __shfl_xor_sync(0xffffffffu, w, 8);
         const int kw = k / 128;
-        if ((lane & 15) == 0 && kw < kt)
+        if ((lane & 7) == 0 && kw < kt)
           *reinterpret_cast<uint32_t*>(tiles + (int64_t)kw * 512 + (r & 31) * 16 + (r >> 5) * 4) = w;
       }
     }
@@ -212,7 +242,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
 }
 
 // ----------------------------------------------------------------------------
-// read-back: the same split, 8 codes of a row per lane and step
+// read-back: the same split, 16 codes of a row per lane and step
 
 __device__ __forceinline__ void decode8(uint32_t codes, float scale, float (&v)[8]) {
   uint32_t h[4];
@@ -233,22 +263,21 @@ __device__ __forceinline__ void decode8(uint32_t codes, float scale, float (&v)[
 __device__ __forceinline__ float scale_value(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte ? byte << 23 : 1u << 22);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                            pack_bf16x2(v[6], v[7]));
+// Eight values into a's words of the output type.
+__device__ __forceinline__ void pack8(__nv_bfloat16, const float (&v)[8], uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
 }
-__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
-  uint32_t w[4];
+__device__ __forceinline__ void pack8(__half, const float (&v)[8], uint32_t* w) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
     w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ void pack8(float, const float (&v)[8], uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
 }
 
 template <typename T>
@@ -266,24 +295,30 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
   for (int r = strip * kStrip + warp; r < min(rows, (strip + 1) * kStrip); r += 8) {
     const int64_t row = row0 + r;
     const uint8_t* srow = tiles + (r & 31) * 16 + (r >> 5) * 4;
-    for (int k0 = lane * 8; k0 < K; k0 += 256 * kAhead) {
-      uint32_t codes[kAhead];
-      uint32_t byte[kAhead];
+    for (int base = lane * 16; base < K; base += kStep * kAheadBack) {
+      uint2 codes[kAheadBack];
+      uint32_t byte[kAheadBack];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int k = k0 + i * 256;
+      for (int i = 0; i < kAheadBack; ++i) {
+        const int k = base + i * kStep;
         if (k < K) {
-          codes[i] = __ldg(reinterpret_cast<const uint32_t*>(packed + (row * K + k) / 2));
+          codes[i] = __ldg(reinterpret_cast<const uint2*>(packed + (row * K + k) / 2));
           byte[i] = __ldg(srow + (int64_t)(k / 128) * 512 + (k / 32) % 4);
         }
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int k = k0 + i * 256;
+      for (int i = 0; i < kAheadBack; ++i) {
+        const int k = base + i * kStep;
         if (k >= K) break;
+        const float sc = scale_value(byte[i]);
+        uint32_t w[sizeof(T) * 4];
         float v[8];
-        decode8(codes[i], scale_value(byte[i]), v);
-        store8(dst + row * K + k, v);
+        decode8(codes[i].x, sc, v);
+        pack8(T(), v, w);
+        decode8(codes[i].y, sc, v);
+        pack8(T(), v, w + sizeof(T) * 2);
+        stg256(dst + row * K + k, w);
+        if constexpr (sizeof(T) == 4) stg256(dst + row * K + k + 8, w + 8);
       }
     }
   }
@@ -316,7 +351,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 // tile's MMAs run.
 //
 // Warps: 0 TMA producer of codes, 1 MMA issuer (the leader CTA's), 2 TMA producer of
-// scales, 4..7 scales to TMEM, 8..15 epilogue (two per TMEM lane quarter).
+// scales, 3 unit scheduler, 4..7 scales to TMEM, 8..15 epilogue (two per TMEM lane
+// quarter).
 enum Mode { GATEUP = 0, DOWN = 1 };
 
 constexpr int BM = 128;
@@ -325,6 +361,7 @@ constexpr int TN = 256;
 constexpr int BKE = 256;           // elements of K per k-block
 constexpr int A_BUFS = 8;          // most k-blocks of A in shared memory
 constexpr int B_STAGES = 8;        // most stages of B (and TMEM scale slots)
+constexpr int U_RING = 4;          // decoded units ahead of their use
 constexpr uint32_t A_BYTES = BM * 128;
 constexpr uint32_t B_BYTES = (TN / 2) * 128;
 constexpr uint32_t SF_BYTES = 3 * 1024;  // two K tiles of this CTA's 128 rows and of both 128-column halves
@@ -365,12 +402,14 @@ struct alignas(16) Smem {
   uint64_t b_full[B_STAGES];    // leader: both CTAs' bytes and scale warps
   uint64_t b_empty[B_STAGES];
   uint64_t sf_full[B_STAGES];   // this CTA's scale bytes
+  uint64_t u_full[U_RING];
+  uint64_t u_empty[U_RING];
   uint64_t tfull;
   uint64_t tempty;              // leader: both CTAs' epilogue warps
   uint32_t tmem_base;
   int abort_flag;
-  int segs;                     // followed by row_start, tile_prefix, blk_prefix [segs + 1]
-  int pad;
+  int4 units[U_RING][2];        // decoded units: {row, end, expert, scale block}, {n0, n1, more, -}
+  // followed by row_start, tile_prefix, blk_prefix [segs + 1]
 };
 struct Table {  // the segment table behind Smem
   int* row_start;
@@ -429,6 +468,13 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// Bring a box of a tensor map into L2.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -484,10 +530,23 @@ __device__ __forceinline__ void build_segments(const Table& tb, const int32_t* o
   }
 }
 
-// Unit u: a row tile and a run of column tiles.  Runs are the outer index, so
-// that the pairs at work together share experts' B tiles in L2.
+struct Ring {  // position in a ring of buffers
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++i == size) i = 0, phase ^= 1;
+  }
+};
+
+// A unit of work: a row tile and a run of column tiles.  Unit u is run u / tiles of row
+// tile u % tiles, so that the pairs at work together share experts' B tiles in L2.
+// One warp decodes units ahead of their use into a ring of shared memory: decoding in
+// every role cost 2 us at each change of unit.
 struct Unit {
-  int seg, m, n0, n1;
+  int row, end;  // first row of the pair's tile, end of its segment
+  int expert;
+  int blk;       // first of the tile's two scale blocks
+  int n0, n1;
 };
 __device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Params& p) {
   const int tiles = tb.tile_prefix[p.segs];
@@ -498,16 +557,24 @@ __device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Params
     if (tb.tile_prefix[mid] <= mt) lo = mid;
     else hi = mid;
   }
-  return Unit{lo, mt - tb.tile_prefix[lo], run * p.n_run, min(p.n_tiles, (run + 1) * p.n_run)};
+  const int m = mt - tb.tile_prefix[lo];
+  return Unit{tb.row_start[lo] + m * TILE_M, tb.row_start[lo + 1], lo % p.experts, tb.blk_prefix[lo] + 2 * m,
+              run * p.n_run, min(p.n_tiles, (run + 1) * p.n_run)};
 }
-
-struct Ring {  // position in a ring of buffers
-  int i = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next(int size) {
-    if (++i == size) i = 0, phase ^= 1;
+// The next unit, false after the last one (or a wait that gave up).  `lanes` of the
+// warp call it together; the first of them frees the slot.
+__device__ __forceinline__ bool next_unit(Smem& sm, Ring& r, Unit& u, int site) {
+  if (!mbar_wait(&sm.u_full[r.i], r.phase, site)) {
+    *(volatile int*)&sm.abort_flag = 1;
+    return false;
   }
-};
+  const int4 a = sm.units[r.i][0], b = sm.units[r.i][1];
+  u = Unit{a.x, a.y, a.z, a.w, b.x, b.y};
+  __syncwarp(__activemask());
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&sm.u_empty[r.i]);
+  r.next(U_RING);
+  return b.z != 0 && !*(volatile int*)&sm.abort_flag;
+}
 
 template <int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -529,7 +596,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  const int first_unit = (int)(blockIdx.x >> 1), num_pairs = (int)(gridDim.x >> 1);
 
   build_segments(tb, p.offsets, p.segs, p.S, 710 + MODE);
   if (warp == 1) {
@@ -542,6 +608,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_init(&sm.b_full[i], 1 + 2 * 4);  // the leader's producer, and the scale warps of both CTAs
         mbar_init(&sm.b_empty[i], 1);
         mbar_init(&sm.sf_full[i], 1);
+      }
+      for (int i = 0; i < U_RING; ++i) {
+        mbar_init(&sm.u_full[i], 1);
+        // two producers, four scale warps, the epilogue, and the leader's MMA issuer
+        mbar_init(&sm.u_empty[i], 2 + 4 + EPI_WARPS + (leader ? 1 : 0));
       }
       mbar_init(&sm.tfull, 1);
       mbar_init(&sm.tempty, 2 * EPI_WARPS);
@@ -569,21 +640,45 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   const uint32_t tmem = sm.tmem_base;
   if (tmem != 0 && threadIdx.x == 0) device_fail(MIRAI_ERR_DEVICE_BOUNDS, 715);  // cannot be: see the MMA issuer
-  const int num_units = tb.tile_prefix[p.segs] * ((p.n_tiles + p.n_run - 1) / p.n_run);
   const int num_kb = (p.K + BKE - 1) / BKE;
   const int total_kb = num_kb + p.has_ext;
   volatile int* abort_flag = &sm.abort_flag;
 
   if (warp < SF_FIRST) {
     regs_dec<REG_LOW>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 3 && lane == 0) {
+      // ======================= unit scheduler =======================
+      const int pairs = (int)(gridDim.x >> 1);
+      const int num_units = tb.tile_prefix[p.segs] * ((p.n_tiles + p.n_run - 1) / p.n_run);
+      Ring r;
+      for (int u = (int)(blockIdx.x >> 1);; u += pairs) {
+        const bool more = u < num_units;
+        Unit un = {};
+        if (more) {
+          un = decode_unit(tb, u, p);
+          // The pairs change row tiles at about the same time: bring the rows into L2 ahead of that
+          // burst (19 MB at 148 SMs).  (Boxes that reach past the last row are left out: prefetching
+          // them took 17 us of a 16-row call.)
+          if (p.resident && un.row + (int)rank * BM + BM <= p.S)
+            for (int kb = 0; kb < num_kb; ++kb) tma_prefetch_2d(&tmap_a, kb * 128, un.row + (int)rank * BM);
+        }
+        if (!mbar_wait(&sm.u_empty[r.i], r.phase ^ 1, 85)) {
+          *abort_flag = 1;
+          break;
+        }
+        sm.units[r.i][0] = make_int4(un.row, un.end, un.expert, un.blk);
+        sm.units[r.i][1] = make_int4(un.n0, un.n1, more, 0);
+        mbar_arrive(&sm.u_full[r.i]);
+        r.next(U_RING);
+        if (!more) break;
+      }
+    } else if (warp == 0 && lane == 0) {
       // ======================= TMA producer =======================
       const uint32_t a_full0 = mapa_shared(smem_u32(&sm.a_full[0]), 0), b_full0 = mapa_shared(smem_u32(&sm.b_full[0]), 0);
-      Ring ra, rb;
-      for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
-        const Unit un = decode_unit(tb, u, p);
-        const int e = un.seg % p.experts;
-        const int row = tb.row_start[un.seg] + un.m * TILE_M + (int)rank * BM;
+      Ring ra, rb, ru;
+      Unit un;
+      while (next_unit(sm, ru, un, 80)) {
+        const int e = un.expert, row = un.row + (int)rank * BM;
         const CUtensorMap* mb = MODE == GATEUP && rank ? &tmap_b1 : &tmap_b0;
         for (int n = un.n0; n < un.n1 && !*abort_flag; ++n) {
           const int brow = e * p.N + (MODE == GATEUP ? n * BM : n * TN + (int)rank * BM);  // B rows of this CTA
@@ -620,11 +715,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else if (warp == 2 && lane == 0) {
       // ======================= TMA producer of the scales =======================
-      Ring rb;
-      for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
-        const Unit un = decode_unit(tb, u, p);
-        const int e = un.seg % p.experts;
-        const int ablk = tb.blk_prefix[un.seg] + un.m * 2 + (int)rank;
+      Ring rb, ru;
+      Unit un;
+      while (next_unit(sm, ru, un, 81)) {
+        const int e = un.expert, ablk = un.blk + (int)rank;
         for (int n = un.n0; n < un.n1 && !*abort_flag; ++n) {
           // row tiles of both column halves
           const int bblk = e * p.w_blocks + (MODE == GATEUP ? n : 2 * n);
@@ -656,19 +750,23 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint32_t id0 = idesc_mxf4(TILE_M, TN, 0), id2 = idesc_mxf4(TILE_M, TN, 2);
       const uint32_t a_lo0 = desc_lo(smem_u32(sA)), b_lo0 = desc_lo(smem_u32(sB));
       const int last_steps = (p.K - (num_kb - 1) * BKE + 63) / 64;  // K = 64 steps of the last k-block
-      Ring ra, rb;
+      Ring ra, rb, ru;
+      Unit un;
       constexpr uint32_t acc = 0;  // all 512 columns are this CTA's: they start at 0 (checked above)
       uint32_t tiles = 0;
       bool ok = true;
-      for (int u = first_unit; u < num_units && ok && !*abort_flag; u += num_pairs) {
-        const Unit un = decode_unit(tb, u, p);
+      while (ok && next_unit(sm, ru, un, 82)) {
         const Ring ra0 = ra;
         for (int n = un.n0; n < un.n1 && ok; ++n, ++tiles) {
           if (p.resident) ra = ra0;
           const bool first = n == un.n0 || !p.resident, last = n + 1 == un.n1 || !p.resident;
-          if (tiles > 0 && !mbar_wait(&sm.tempty, (tiles - 1) & 1, 74)) ok = false;
+          // (the first k-block's operands are waited for before the accumulator: they come first)
+          if ((first && !mbar_wait(&sm.a_full[ra.i], ra.phase, 75)) || !mbar_wait(&sm.b_full[rb.i], rb.phase, 76) ||
+              (tiles > 0 && !mbar_wait(&sm.tempty, (tiles - 1) & 1, 74)))
+            ok = false;
           for (int kb = 0; kb < total_kb && ok; ++kb) {
-            if ((first && !mbar_wait(&sm.a_full[ra.i], ra.phase, 75)) || !mbar_wait(&sm.b_full[rb.i], rb.phase, 76)) {
+            if (kb > 0 && ((first && !mbar_wait(&sm.a_full[ra.i], ra.phase, 75)) ||
+                           !mbar_wait(&sm.b_full[rb.i], rb.phase, 76))) {
               ok = false;
               break;
             }
@@ -711,9 +809,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     regs_dec<REG_LOW>();
     const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t b_full0 = mapa_shared(smem_u32(&sm.b_full[0]), 0);
-    Ring rb;
-    for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
-      const Unit un = decode_unit(tb, u, p);
+    Ring rb, ru;
+    Unit un;
+    while (next_unit(sm, ru, un, 83)) {
       const int blocks = (un.n1 - un.n0) * total_kb;
       int kb = 0;
       for (int i = 0; i < blocks; ++i) {
@@ -750,11 +848,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t box_row = smem_u32(box) + (uint32_t)lane * 64u;
     const uint32_t box_sw = (uint32_t)(lane >> 1) & 3u;  // 64-byte swizzle: 16-byte chunk ^= row bits 1..2
     uint32_t tiles = 0;
-    for (int u = first_unit; u < num_units && !*abort_flag; u += num_pairs) {
-      const Unit un = decode_unit(tb, u, p);
-      const int local = un.m * TILE_M + (int)rank * BM + q * 32 + lane;
-      const int64_t row = (int64_t)tb.row_start[un.seg] + local;
-      const bool valid = row < tb.row_start[un.seg + 1];
+    Ring ru;
+    Unit un;
+    while (next_unit(sm, ru, un, 84)) {
+      const int64_t row = (int64_t)un.row + (int)rank * BM + q * 32 + lane;
+      const bool valid = row < un.end;
       const bool boxed = __all_sync(0xffffffffu, valid);  // all 32 rows are the segment's
       const int row0 = (int)(row - lane);
       // 32 rows x 32 columns: through the staging box and one TMA store, or row by row.  (A lane
@@ -837,7 +935,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 codes[x] = byte == 255u ? 0u : e2m1x8(f);
               }
               *reinterpret_cast<uint4*>(p.hq + (row * p.N + col) / 2) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-              const int64_t blk = tb.blk_prefix[un.seg] + un.m * 2 + (int)rank;
+              const int64_t blk = un.blk + (int)rank;
               if (blk < p.h_blocks) {
                 uint8_t* word = p.hscale + (blk * p.h_kt + n) * 512 + lane * 16 + q * 4;
                 word[c] = (uint8_t)byte;
@@ -1086,7 +1184,7 @@ size_t mirai_mxfp4_rows_scale_bytes(int64_t num_rows, int32_t num_segments, int3
 int mirai_mxfp4_quantize(const void* weight, int32_t dtype, int32_t num_experts, int64_t out_features,
                          int64_t in_features, uint8_t* packed, uint8_t* scale, mirai_stream_t stream) {
   if (int rc = mx::matrix_problem("mxfp4_quantize", num_experts, out_features, in_features)) return rc;
-  if (!weight || !packed || !scale || mx::misaligned(weight) || mx::misaligned(packed) || mx::misaligned(scale))
+  if (!weight || !packed || !scale || mx::misaligned(weight, 32) || mx::misaligned(packed) || mx::misaligned(scale))
     return set_error(MIRAI_ERR_INVALID_ARG, "mxfp4_quantize: null or misaligned pointer");
   const int64_t grid = mx::strips("mxfp4_quantize", num_experts * mx::ceil_div(out_features, mx::kBlockRows));
   if (grid < 0) return MIRAI_ERR_UNSUPPORTED;
@@ -1106,7 +1204,7 @@ int mirai_mxfp4_quantize(const void* weight, int32_t dtype, int32_t num_experts,
 int mirai_mxfp4_dequantize(const uint8_t* packed, const uint8_t* scale, int32_t num_experts, int64_t out_features,
                            int64_t in_features, void* out, int32_t dtype, mirai_stream_t stream) {
   if (int rc = mx::matrix_problem("mxfp4_dequantize", num_experts, out_features, in_features)) return rc;
-  if (!out || !packed || !scale || mx::misaligned(out) || mx::misaligned(packed) || mx::misaligned(scale))
+  if (!out || !packed || !scale || mx::misaligned(out, 32) || mx::misaligned(packed) || mx::misaligned(scale))
     return set_error(MIRAI_ERR_INVALID_ARG, "mxfp4_dequantize: null or misaligned pointer");
   const int64_t grid = mx::strips("mxfp4_dequantize", num_experts * mx::ceil_div(out_features, mx::kBlockRows));
   if (grid < 0) return MIRAI_ERR_UNSUPPORTED;
@@ -1136,7 +1234,7 @@ int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_
   if (!row_index && x_rows < num_rows)
     return set_error(MIRAI_ERR_INVALID_ARG, "mxfp4_quantize_rows: %lld input rows for %lld rows", (long long)x_rows,
                      (long long)num_rows);
-  if (!x || !offsets || !packed || !scale || mx::misaligned(x) || mx::misaligned(packed) || mx::misaligned(scale))
+  if (!x || !offsets || !packed || !scale || mx::misaligned(x, 32) || mx::misaligned(packed) || mx::misaligned(scale))
     return set_error(MIRAI_ERR_INVALID_ARG, "mxfp4_quantize_rows: null or misaligned pointer");
   const int64_t grid = mx::strips("mxfp4_quantize_rows", mx::max_blocks(num_rows, num_segments));
   if (grid < 0) return MIRAI_ERR_UNSUPPORTED;

@@ -359,8 +359,8 @@ def _same_device(device: torch.device, **tensors) -> None:
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` at a 16-byte aligned address (a copy when a view starts elsewhere)."""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    """``t`` at a 32-byte aligned address (a copy when a view starts elsewhere)."""
+    return t if t.data_ptr() % 32 == 0 else t.clone()
 
 
 def _tiles(rows: int, width: int) -> tuple[int, int]:
@@ -477,9 +477,9 @@ def mxfp4_dequantize(w: Mxfp4Tensor, out: torch.Tensor | None = None,
         if out_dtype not in _MXFP4_DTYPES:
             raise TypeError(f"mxfp4_dequantize writes bf16, fp32 or fp16, not {out_dtype}")
         out = torch.empty(w.shape, dtype=out_dtype, device=w.packed.device)
-    if out.dtype not in _MXFP4_DTYPES or tuple(out.shape) != w.shape or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {w.shape} tensor of bf16, fp32 or fp16, got {out.dtype} "
-                         f"{tuple(out.shape)}")
+    if out.dtype not in _MXFP4_DTYPES or tuple(out.shape) != w.shape or not out.is_contiguous() or out.data_ptr() % 32:
+        raise ValueError(f"out must be a contiguous, 32-byte aligned {w.shape} tensor of bf16, fp32 or fp16, got "
+                         f"{out.dtype} {tuple(out.shape)}")
     _same_device(w.packed.device, out=out)
     E, out_f, in_f = w.shape
     with torch.cuda.device(out.device):
