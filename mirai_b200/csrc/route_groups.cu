@@ -8,14 +8,18 @@
 //
 // Decisions are those of 64-bit arithmetic: a row is decided in fp32 together
 // with a bound on the fp32 error, and a row where two compared values lie within
-// it (about one in a thousand) is decided again in 64 bits by the same code.
-// Without a bias, experts and group maxima are ranked by the logits themselves,
-// which is exact.
+// it (a few in a thousand) is decided again in 64 bits.  Without a bias, experts
+// and group maxima are ranked by the logits themselves, which is exact.
 //
 // W lanes hold a token's experts, so a warp routes 32 / W tokens: each group on
 // whole lanes (a power of two of them), PER experts per lane, so that expert
 // order is lane order, group scores are butterflies inside a group, and ties
 // resolve to the lowest lane.
+//
+// route_fast (up to 32 experts per lane) ranks 32-bit words of the key's leading bits
+// and the expert's id: a lane sorts its words by a network of integer minima and
+// maxima, and k + 1 rounds take the largest head.  What it cannot decide, the whole
+// warp decides one row after the other in 64 bits (route_exact).
 #include "common.cuh"
 
 namespace mirai {
@@ -33,7 +37,11 @@ struct Args {
   int gs;       // experts per group
   int shift;    // log2 of the lanes per group
   int per;      // experts per lane, <= PER
+  int shift32, per32;  // the same with a whole warp per token
   int score;    // MIRAI_SCORE_*
+  int vec;      // rows can be read 16 bytes at a time
+  int vec_bias;
+  int id_bits;  // bits of an expert id
   int top2;     // group score: 1 the two best scores, 0 the best key
   int norm;     // MIRAI_NORM_*
   float scale;
@@ -94,13 +102,82 @@ template <typename F> __device__ __forceinline__ void denominator(int norm, int 
   if (sum != sum) den = sum;  // NaN scores stay NaN
 }
 
-// One token on W lanes.  Returns (fp32 only) whether a comparison was too close
-// to call; otherwise, and always in 64 bits, its slots are written when `write`.
-template <typename F, typename T, int PER, int W>
-__device__ __forceinline__ bool route_row(const Args& a, int64_t t, bool write) {
-  constexpr bool FAST = sizeof(F) == 4;
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// PER consecutive values of a row, -inf past the first n of them.  Whole rows of vectors
+// (vec) are read 16 bytes at a time.
+template <int PER> __device__ __forceinline__ void load_row(const float* p, int n, bool vec, float (&v)[PER]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (i < n) x = __ldg(reinterpret_cast<const float4*>(p + i));
+      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = i < n ? __ldg(p + i) : -INFINITY;
+  }
+}
+template <int PER> __device__ __forceinline__ void load_row(const __nv_bfloat16* p, int n, bool vec, float (&v)[PER]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      uint2 x = make_uint2(0xff80ff80u, 0xff80ff80u);
+      if (i < n) x = __ldg(reinterpret_cast<const uint2*>(p + i));
+      v[i] = bf16_lo(x.x), v[i + 1] = bf16_hi(x.x), v[i + 2] = bf16_lo(x.y), v[i + 3] = bf16_hi(x.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = i < n ? __bfloat162float(p[i]) : -INFINITY;
+  }
+}
+
+// Descending order by compare-exchanges that no data decides: Batcher's odd-even
+// merge sort (19 exchanges of 8 words, 63 of 16).
+template <int N> __device__ __forceinline__ void sort_desc(uint32_t (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2) {
+#pragma unroll
+    for (int q = p; q > 0; q /= 2) {
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q) {
+#pragma unroll
+        for (int i = 0; i < q; ++i) {
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t hi = max(v[i + j], v[i + j + q]), lo = min(v[i + j], v[i + j + q]);
+            v[i + j] = hi, v[i + j + q] = lo;
+          }
+        }
+      }
+    }
+  }
+}
+
+// The larger one; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// One token on W lanes, by leading bits.  Returns whether the next stage has to decide
+// it (a comparison too close to call, or a NaN in the row); otherwise the slots are
+// written when `write`.
+template <typename T, int PER, int W>
+__device__ __forceinline__ bool route_fast(const Args& a, int64_t t, bool write) {
   constexpr int SLOTS = (kMaxTopK + W - 1) / W;
-  const F kLow = -INFINITY;
+  const float kLow = -INFINITY;
   const int lane = threadIdx.x & 31;
   const int li = lane & (W - 1);
   const int first_lane = lane & ~(W - 1);
@@ -109,83 +186,222 @@ __device__ __forceinline__ bool route_row(const Args& a, int64_t t, bool write) 
   const int in_group = (li & ((1 << a.shift) - 1)) * a.per;
   const int e0 = group * a.gs + in_group;
   const int n = group < a.G ? max(0, min(a.per, a.gs - in_group)) : 0;
+  const T* row = static_cast<const T*>(a.logits) + t * a.E;
+  const bool soft = a.score == MIRAI_SCORE_SOFTMAX;
+  const bool scored = a.bias || (a.top2 && a.top_groups < a.G);  // scores take part in the choice
+
+  float key[PER];
+  load_row<PER>(row + e0, n, a.vec, key);
+  float mx = kLow;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mx = max_nan(mx, key[i]);
+  bool close = mx != mx;
+  float smax = 1.f, inv = 1.f;
+  float best1 = kLow, best2 = kLow;
+  if (soft) {
+    mx = max_lanes<W>(mx);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += key[i] == kLow ? 0.f : ex2((key[i] - mx) * kLog2e);
+    sum = sum_lanes<W>(sum);
+    inv = sum == 0.f ? 0.f : 1.f / sum;
+    smax = inv;
+  }
+  if (scored) {
+    float bias[PER];
+    if (a.bias) load_row<PER>(a.bias + e0, n, a.vec_bias, bias);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool open = key[i] != kLow;
+      float v = soft ? ex2((key[i] - mx) * kLog2e) * inv : rcp(1.f + ex2(key[i] * -kLog2e));
+      if (a.bias) {
+        v = open ? v + bias[i] : kLow;
+        v = fmaxf(v, kLow);  // (a NaN bias closes its expert)
+        key[i] = v;
+      } else {
+        v = open ? v : kLow;
+      }
+      best2 = fmaxf(best2, fminf(best1, v));
+      best1 = fmaxf(best1, v);
+    }
+  }
+  if (!a.top2) {
+    best1 = kLow;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best1 = fmaxf(best1, key[i]);
+  }
+  // Error of a score: ex2 and rcp are within 2^-22 of their values and the exponent's product
+  // adds |x| 2^-24, times s (1 - s) <= 1/4 (and <= 0.23 / |x|), with two roundings of s: below
+  // 2^-21.9 for sigmoid; softmax as in route_row.
+  const float score_err = smax * (soft ? 0x1p-17f : 0x1.8p-22f);
+  bool stays = group < a.G;
+  if (a.top_groups < a.G) {
+    for (int o = 1 << a.shift >> 1; o > 0; o >>= 1) {
+      const float o1 = __shfl_xor_sync(0xffffffffu, best1, o), o2 = __shfl_xor_sync(0xffffffffu, best2, o);
+      best2 = fmaxf(fmaxf(best2, o2), fminf(best1, o1));
+      best1 = fmaxf(best1, o1);
+    }
+    const float gv = a.top2 && best2 != kLow ? best1 + best2 : best1;
+    int rank = 0;
+    for (int g = 0; g < a.G; ++g) {
+      const float v = __shfl_sync(0xffffffffu, gv, first_lane + (g << a.shift));
+      rank += v > gv || (v == gv && g < group);
+    }
+    stays = stays && rank < a.top_groups;
+    if (scored) {
+      const uint32_t in = __ballot_sync(0xffffffffu, group < a.G && rank == a.top_groups - 1) & team;
+      const uint32_t out = __ballot_sync(0xffffffffu, group < a.G && rank == a.top_groups) & team;
+      const float worst_in = __shfl_sync(0xffffffffu, gv, __ffs(in) - 1);
+      const float best_out = __shfl_sync(0xffffffffu, gv, __ffs(out) - 1);
+      if (best_out != kLow)
+        close |= worst_in - best_out <= 4.f * score_err + 0x1p-21f * (fabsf(worst_in) + fabsf(best_out) + smax);
+    }
+  }
+  // leading bits of the key, then the id (lowest first), 0 for a closed slot
+  const uint32_t ids = (1u << a.id_bits) - 1u;
+  uint32_t v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v[i] = i < n && stays ? (order(key[i]) & ~ids) | (ids - (uint32_t)(e0 + i)) : 0u;
+  sort_desc<PER>(v);
+  int slot[SLOTS];
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) slot[m] = 0;
+  uint32_t last = 0;  // the word of slot k - 1, then the first one left out
+  for (int j = 0; j <= a.k; ++j) {
+    const uint32_t top = max_lanes<W>(v[0]);
+    if (j == a.k) {
+      // The cut: one word stands for every key left out, so equal (or, with the keys' errors,
+      // too near) leading bits leave it open.  Among -inf the id decides.
+      const uint32_t up = top | ids, above = last & ~ids;
+      if (top && up != 0x007fffffu) {
+        const float lo = __uint_as_float(above & 0x80000000u ? above & 0x7fffffffu : ~above);
+        const float x = __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
+        close |= up >= above || (a.bias && lo - x <= 2.f * score_err + 0x1p-22f * fabsf(x));
+      }
+      break;
+    }
+    last = top;
+#pragma unroll
+    for (int m = 0; m < SLOTS; ++m)
+      if (j == m * W + li) slot[m] = (int)(ids - (top & ids));
+    const bool pop = v[0] == top;
+#pragma unroll
+    for (int i = 0; i + 1 < PER; ++i) v[i] = pop ? v[i + 1] : v[i];
+    v[PER - 1] = pop ? 0u : v[PER - 1];
+  }
+  // The slots' scores again, from their logits; their order by the whole key.
+  float s[SLOTS], full[SLOTS], total = 0.f;
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) {
+    s[m] = 0.f;
+    full[m] = kLow;
+    if (m * W + li < a.k) {
+      const float x = load_logit(row + slot[m]);
+      if (x == x && x != kLow) {
+        s[m] = soft ? expf(x - mx) * inv : 1.f / (1.f + expf(-x));
+        full[m] = a.bias ? fmaxf(s[m] + __ldg(a.bias + slot[m]), kLow) : x;
+      }
+    }
+    total += s[m];
+  }
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) {
+    // the slot after this one: the next lane's, or the first lane's next
+    const float same = __shfl_sync(0xffffffffu, full[m], first_lane + ((li + 1) & (W - 1)));
+    const float wrap = __shfl_sync(0xffffffffu, full[m + 1 < SLOTS ? m + 1 : m], first_lane);
+    const int id_same = __shfl_sync(0xffffffffu, slot[m], first_lane + ((li + 1) & (W - 1)));
+    const int id_wrap = __shfl_sync(0xffffffffu, slot[m + 1 < SLOTS ? m + 1 : m], first_lane);
+    const float next = li + 1 < W ? same : wrap;
+    const int id = li + 1 < W ? id_same : id_wrap;
+    if (m * W + li + 1 < a.k && next != kLow) {
+      if (a.bias) close |= full[m] - next <= 2.f * score_err + 0x1p-22f * fabsf(next);
+      else close |= next > full[m] || (next == full[m] && id < slot[m]);
+    }
+  }
+  close = (__ballot_sync(0xffffffffu, close) & team) != 0;  // (no early return: shuffles take the whole warp)
+  total = sum_lanes<W>(total);
+  float den, scale;
+  bool follows;
+  denominator(a.norm, a.k, a.scale, total, den, scale, follows);
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) {
+    const int j = m * W + li;
+    if (j >= a.k || !write || close) continue;
+    a.idx[t * a.k + j] = slot[m];
+    a.w[t * a.k + j] = s[m] / den * scale;
+  }
+  return close;
+}
+
+// One token on the whole warp, in 64 bits.
+template <typename T, int PER>
+__device__ __forceinline__ void route_exact(const Args& a, int64_t t) {
+  using O = uint64_t;
+  const double kLow = -INFINITY;
+  const int lane = threadIdx.x & 31;
+  const int group = lane >> a.shift32;
+  const int in_group = (lane & ((1 << a.shift32) - 1)) * a.per32;
+  const int e0 = group * a.gs + in_group;
+  const int n = group < a.G ? max(0, min(a.per32, a.gs - in_group)) : 0;
   const T* row = static_cast<const T*>(a.logits) + t * a.E + e0;
 
-  F key[PER], sc[PER];  // ranking key (-inf: closed by its logit) and score
-  F mx = kLow;
+  double key[PER], sc[PER];  // ranking key (-inf: closed by its logit) and score
+  double mx = kLow;
   bool nan = false;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const F l = i < n ? F(load_logit(row + i)) : kLow;
+    const double l = i < n ? (double)load_logit(row + i) : kLow;
     nan |= l != l;
     key[i] = l != l ? kLow : l;
     mx = key[i] > mx ? key[i] : mx;
   }
-  nan = (__ballot_sync(0xffffffffu, nan) & team) != 0;
-  F smax = F(1);  // bounds every score
+  nan = __any_sync(0xffffffffu, nan);
   if (a.score == MIRAI_SCORE_SOFTMAX) {
-    mx = max_lanes<W>(mx);
-    F sum = F(0);
+    mx = max_lanes<32>(mx);
+    double sum = 0.;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      sc[i] = key[i] == kLow ? F(0) : real_exp(key[i] - mx);
+      sc[i] = key[i] == kLow ? 0. : exp(key[i] - mx);
       sum += sc[i];
     }
-    sum = sum_lanes<W>(sum);
-    smax = sum == F(0) ? F(0) : F(1) / sum;
+    sum = sum_lanes<32>(sum);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sc[i] *= smax;
+    for (int i = 0; i < PER; ++i) sc[i] = sum == 0. ? 0. : sc[i] / sum;
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sc[i] = key[i] == kLow ? F(0) : F(1) / (F(1) + real_exp(-key[i]));
+    for (int i = 0; i < PER; ++i) sc[i] = key[i] == kLow ? 0. : 1. / (1. + exp(-key[i]));
   }
-  // Error of a score: sigmoid within 4 roundings of a value <= 1; softmax within 70
-  // (its sum) of a value <= smax.  A bias adds half a unit of the key.
-  const F score_err = smax * (a.score == MIRAI_SCORE_SOFTMAX ? F(0x1p-17f) : F(0x1p-21f));
-  bool close = false;
-
   // group scores; without a bias they compare the scores' sums, or the logits
-  F best1 = kLow, best2 = kLow;
+  double best1 = kLow, best2 = kLow;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const bool open = key[i] != kLow;
     if (a.bias) {
-      const F b = F(i < n ? __ldg(a.bias + e0 + i) : 0.f);
-      key[i] = open ? sc[i] + b : kLow;
+      key[i] = open ? sc[i] + (double)(i < n ? __ldg(a.bias + e0 + i) : 0.f) : kLow;
       if (key[i] != key[i]) key[i] = kLow;
     }
-    const F v = a.top2 ? (open ? (a.bias ? key[i] : sc[i]) : kLow) : key[i];
+    const double v = a.top2 ? (open ? (a.bias ? key[i] : sc[i]) : kLow) : key[i];
     if (v > best1) best2 = best1, best1 = v;
     else if (v > best2) best2 = v;
   }
-  bool stays = true;  // this lane's group is among the best
+  bool stays = group < a.G;  // this lane's group is among the best
   if (a.top_groups < a.G) {
-    for (int o = 1 << a.shift >> 1; o > 0; o >>= 1) {
-      const F o1 = __shfl_xor_sync(0xffffffffu, best1, o), o2 = __shfl_xor_sync(0xffffffffu, best2, o);
-      const F low = best1 < o1 ? best1 : o1;
+    for (int o = 1 << a.shift32 >> 1; o > 0; o >>= 1) {
+      const double o1 = __shfl_xor_sync(0xffffffffu, best1, o), o2 = __shfl_xor_sync(0xffffffffu, best2, o);
+      const double low = best1 < o1 ? best1 : o1;
       best1 = best1 < o1 ? o1 : best1;
       best2 = best2 < o2 ? o2 : best2;
       best2 = best2 < low ? low : best2;
     }
-    const F gv = a.top2 && best2 != kLow ? best1 + best2 : best1;
+    const double gv = a.top2 && best2 != kLow ? best1 + best2 : best1;
     int rank = 0;
     for (int g = 0; g < a.G; ++g) {
-      const F v = __shfl_sync(0xffffffffu, gv, first_lane + (g << a.shift));
+      const double v = __shfl_sync(0xffffffffu, gv, g << a.shift32);
       rank += v > gv || (v == gv && g < group);
     }
-    stays = group < a.G && rank < a.top_groups;
-    if (FAST && (a.top2 || a.bias)) {  // the last group in against the first one out
-      const uint32_t in = __ballot_sync(0xffffffffu, group < a.G && rank == a.top_groups - 1) & team;
-      const uint32_t out = __ballot_sync(0xffffffffu, group < a.G && rank == a.top_groups) & team;
-      const F worst_in = __shfl_sync(0xffffffffu, gv, __ffs(in) - 1);
-      const F best_out = __shfl_sync(0xffffffffu, gv, __ffs(out) - 1);
-      if (best_out != kLow)
-        close |= worst_in - best_out <= F(4) * score_err + F(0x1p-21f) * (fabs(worst_in) + fabs(best_out) + smax);
-    }
+    stays = stays && rank < a.top_groups;
   }
-
   // top-k: every lane offers its best key; the lowest of the best lanes wins
-  using O = decltype(order(F(0)));
   uint32_t open_mask[(PER + 31) / 32];
 #pragma unroll
   for (int m = 0; m < (PER + 31) / 32; ++m) open_mask[m] = 0;
@@ -194,7 +410,7 @@ __device__ __forceinline__ bool route_row(const Args& a, int64_t t, bool write) 
     if (i < n && stays) open_mask[i / 32] |= 1u << (i & 31);
   O best = 0;
   int best_i = 0;
-  F best_s = F(0);
+  double best_s = 0.;
   auto rescan = [&]() {
     best = 0;
 #pragma unroll
@@ -204,29 +420,15 @@ __device__ __forceinline__ bool route_row(const Args& a, int64_t t, bool write) 
     }
   };
   rescan();
-  int slot_e[SLOTS];
-  F slot_s[SLOTS];
-#pragma unroll
-  for (int m = 0; m < SLOTS; ++m) slot_e[m] = 0, slot_s[m] = F(0);
-  F total = F(0), previous = INFINITY;
-  const bool check = FAST && a.bias != nullptr;
-  const F key_err = F(2) * score_err;
-  for (int j = 0; j < a.k + (check ? 1 : 0); ++j) {
-    const O top = max_lanes<W>(best);
-    if (check) {
-      const F v = __uint_as_float(top & 0x80000000u ? (uint32_t)top & 0x7fffffffu : ~(uint32_t)top);
-      if (top && v != kLow) close |= previous - v <= key_err + F(0x1p-22f) * fabs(v);
-      previous = v;
-      if (j == a.k) break;
-    }
-    const uint32_t who = __ballot_sync(0xffffffffu, best == top) & team;
-    const int winner = __ffs(who) - 1;
+  int slot_e = 0;  // lane j: slot j
+  double slot_s = 0., total = 0.;
+  for (int j = 0; j < a.k; ++j) {
+    const O top = max_lanes<32>(best);
+    const int winner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
     const int e = __shfl_sync(0xffffffffu, e0 + best_i, winner);
-    const F s = __shfl_sync(0xffffffffu, best_s, winner);
+    const double s = __shfl_sync(0xffffffffu, best_s, winner);
     total += s;
-#pragma unroll
-    for (int m = 0; m < SLOTS; ++m)
-      if (j == m * W + li) slot_e[m] = e, slot_s[m] = s;
+    if (j == lane) slot_e = e, slot_s = s;
     if (lane == winner) {
 #pragma unroll
       for (int m = 0; m < (PER + 31) / 32; ++m)
@@ -234,108 +436,165 @@ __device__ __forceinline__ bool route_row(const Args& a, int64_t t, bool write) 
       rescan();
     }
   }
-  if (FAST && (__ballot_sync(0xffffffffu, close) & team)) return true;
-  if (!write) return false;
-  F den, scale;
+  double den, scale;
   bool follows;
   denominator(a.norm, a.k, a.scale, total, den, scale, follows);
-#pragma unroll
-  for (int m = 0; m < SLOTS; ++m) {
-    const int j = m * W + li;
-    if (j >= a.k) continue;
-    a.idx[t * a.k + j] = slot_e[m];
-    a.w[t * a.k + j] = nan ? __uint_as_float(0x7fffffffu) : (float)(slot_s[m] / den * scale);
+  if (lane < a.k) {
+    a.idx[t * a.k + lane] = slot_e;
+    a.w[t * a.k + lane] = nan ? __uint_as_float(0x7fffffffu) : (float)(slot_s / den * scale);
   }
-  return false;
 }
 
-// The rows of a warp that fp32 could not decide, in 64 bits (rare: kept out of the fast path's registers).
-template <typename T, int PER, int W> __device__ __noinline__ void route_close_rows(const Args& a, int64_t t, bool write) {
-  route_row<double, T, PER, W>(a, t, write);
+// The warp's rows in `rows` (bit = first lane of the row's team), one after the other
+// (kept out of the fast path's registers).
+template <typename T, int PER, int W>
+__device__ __noinline__ void route_exact_rows(const Args& a, int64_t first, uint32_t rows) {
+  for (; rows; rows &= rows - 1) route_exact<T, PER>(a, first + (__ffs(rows) - 1) / W);
 }
 
-template <typename T, int PER, int W> __global__ void __launch_bounds__(256) route_groups_kernel(const __grid_constant__ Args a) {
+template <typename T, int PER, int W>
+__global__ void __launch_bounds__(256, PER <= 16 ? 4 : (PER <= 32 ? 2 : 1))
+    route_groups_kernel(const __grid_constant__ Args a) {
+  constexpr int PER32 = W < 32 ? 8 : PER;  // experts per lane of a whole warp
   const int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / W;
   const bool live = t < a.T;
-  const int64_t tc = live ? t : a.T - 1;  // lanes past the end repeat the last token, unwritten
-  const bool close = route_row<float, T, PER, W>(a, tc, live);
-  if (__any_sync(0xffffffffu, close)) route_close_rows<T, PER, W>(a, tc, live && close);
+  bool open = true;
+  if constexpr (PER <= 32) open = route_fast<T, PER, W>(a, live ? t : a.T - 1, live);  // past the end: unwritten
+  const int lane = threadIdx.x & 31;
+  const uint32_t rows = __ballot_sync(0xffffffffu, open && live && (lane & (W - 1)) == 0);
+  if (rows) route_exact_rows<T, PER32, W>(a, t - lane / W, rows);
 }
 
 // ----------------------------------------------------------------------------
 // Backward: dL/ds_j = scale (g_j - [den follows] sum_i g_i s_i / den) / den, then
 //   sigmoid  dl_e = ds s (1 - s) at the selected experts, 0 elsewhere
 //   softmax  dl_e = s_e (ds_e - sum_j ds_j s_j)
-// One warp per token: the row is streamed once (softmax) and its gradient
-// written once, zeros or the softmax tail everywhere, then lane j corrects slot j's
-// expert (an index given twice gets the sum of both).
+// W lanes per token (a warp takes 32 / W, since one token's chain of dependent loads is
+// latency): the row is streamed once (softmax) and its gradient written once, zeros or the
+// softmax tail everywhere, then slot j's lane corrects its expert (an index given twice
+// gets the sum of both).  Lanes take vectors of four in turn, so rows move whole.
 __device__ __forceinline__ void store_grad(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_grad(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store4(float* p, const float* v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
 
-template <typename T, int PER>
+template <typename T, int PER, int W>
 __global__ void __launch_bounds__(256) route_groups_backward_kernel(const float* __restrict__ grad_w,
                                                                     const T* __restrict__ logits,
                                                                     const int64_t* __restrict__ idx, int64_t tokens,
-                                                                    int E, int k, int score, int norm,
+                                                                    int E, int k, int score, int norm, int vec,
                                                                     float route_scale, T* __restrict__ out) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (t >= tokens) return;
+  constexpr int SLOTS = (kMaxTopK + W - 1) / W;
+  const int lane = threadIdx.x & 31, li = lane & (W - 1);
+  const int64_t own = ((int64_t)blockIdx.x * 256 + threadIdx.x) / W;
+  const bool live = own < tokens;
+  const int64_t t = live ? own : tokens - 1;  // lanes past the end repeat the last token, unwritten
   const T* row = logits + t * E;
   T* grow = out + t * E;
   const bool soft = score == MIRAI_SCORE_SOFTMAX;
+  // the slots' ids and gradients first: their logits hang on them
+  int e[SLOTS];
+  float g[SLOTS], s[SLOTS], x[SLOTS];
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) {
+    const int j = m * W + li;
+    e[m] = -1;
+    g[m] = x[m] = 0.f;
+    if (j < k) {
+      const int64_t id = idx[t * k + j];
+      g[m] = grad_w[t * k + j];
+      if (id < 0 || id >= E) {
+        if (live) device_fail(MIRAI_ERR_DEVICE_BOUNDS, 750);
+      } else {
+        e[m] = (int)id;
+        x[m] = load_logit(row + id);
+      }
+    }
+  }
   float l[PER];
   float mx = -INFINITY, inv = 0.f;
   if (soft) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = i * 32 + lane;
-      l[i] = e < E ? load_logit(row + e) : -INFINITY;
-      mx = fmaxf(mx, l[i]);
+    for (int i = 0; i < PER; i += 4) {
+      const int c = (i / 4 * W + li) * 4;
+      float v[4];
+      load_row<4>(row + c, E - c, vec, v);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) l[i + z] = v[z], mx = fmaxf(mx, v[z]);
     }
-    mx = max_lanes<32>(mx);
+    mx = max_lanes<W>(mx);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      l[i] = l[i] == -INFINITY ? 0.f : expf(l[i] - mx);  // from here on: the scores
+      l[i] = l[i] == -INFINITY ? 0.f : ex2((l[i] - mx) * kLog2e);  // from here on: the scores
       sum += l[i];
     }
-    sum = sum_lanes<32>(sum);
+    sum = sum_lanes<W>(sum);
     inv = sum == 0.f ? 0.f : 1.f / sum;
   }
-  int64_t e = -1;
-  float s = 0.f, g = 0.f;
-  if (lane < k) {
-    e = idx[t * k + lane];
-    if (e < 0 || e >= E) {
-      device_fail(MIRAI_ERR_DEVICE_BOUNDS, 750);
-      e = -1;
-    } else {
-      const float x = load_logit(row + e);
-      s = x == -INFINITY ? 0.f : (soft ? expf(x - mx) * inv : 1.f / (1.f + expf(-x)));
-      g = grad_w[t * k + lane];
-    }
+  float total = 0.f;
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) {
+    s[m] = e[m] < 0 || x[m] == -INFINITY ? 0.f : (soft ? expf(x[m] - mx) * inv : 1.f / (1.f + expf(-x[m])));
+    total += s[m];
   }
   float den, scale;
   bool follows;
-  denominator(norm, k, route_scale, sum_lanes<32>(s), den, scale, follows);
-  const float mean = follows ? sum_lanes<32>(g * (s / den)) : 0.f;
-  const float ds = e >= 0 ? scale * ((g - mean) / den) : 0.f;
-  float mine = ds * s;  // this slot's share of dL/ds * s, and the same of slots that name its expert
-  const float dot = sum_lanes<32>(mine);
-  float sums = 0.f;
-  for (int j = 0; j < k; ++j) {
-    const int64_t other = __shfl_sync(0xffffffffu, e, j);
-    const float v = __shfl_sync(0xffffffffu, mine, j);
-    if (other == e) sums += v;
-  }
+  denominator(norm, k, route_scale, sum_lanes<W>(total), den, scale, follows);
+  float mean = 0.f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int x = i * 32 + lane;
-    if (x < E) store_grad(grow + x, soft ? -(l[i] * inv) * dot : 0.f);
+  for (int m = 0; m < SLOTS; ++m)
+    if (e[m] >= 0) mean += g[m] * (s[m] / den);
+  mean = sum_lanes<W>(mean);  // (by the whole warp: the tokens of one may differ in `follows`)
+  if (!follows) mean = 0.f;
+  float mine[SLOTS], dot = 0.f;  // dL/ds * s of each slot
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) {
+    mine[m] = e[m] >= 0 ? scale * ((g[m] - mean) / den) * s[m] : 0.f;
+    dot += mine[m];
+  }
+  dot = sum_lanes<W>(dot);
+  // slots that name the same expert share the sum of theirs
+  float sums[SLOTS];
+#pragma unroll
+  for (int m = 0; m < SLOTS; ++m) sums[m] = 0.f;
+#pragma unroll
+  for (int m2 = 0; m2 < SLOTS; ++m2) {
+    for (int j = 0; j < W && m2 * W + j < k; ++j) {
+      const int other = __shfl_sync(0xffffffffu, e[m2], (lane & ~(W - 1)) + j);
+      const float v = __shfl_sync(0xffffffffu, mine[m2], (lane & ~(W - 1)) + j);
+#pragma unroll
+      for (int m = 0; m < SLOTS; ++m)
+        if (other == e[m]) sums[m] += v;
+    }
+  }
+  const float tail = -inv * dot;
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      const int c = (i / 4 * W + li) * 4;
+      float v[4];
+#pragma unroll
+      for (int z = 0; z < 4; ++z) v[z] = soft ? l[i + z] * tail : 0.f;
+      if (vec) {
+        if (c < E) store4(grow + c, v);
+      } else {
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (c + z < E) store_grad(grow + c + z, v[z]);
+      }
+    }
   }
   __syncwarp();
-  if (e >= 0) store_grad(grow + e, soft ? sums - s * dot : sums * (1.f - s));
+  if (live) {
+#pragma unroll
+    for (int m = 0; m < SLOTS; ++m)
+      if (e[m] >= 0) store_grad(grow + e[m], soft ? sums[m] - s[m] * dot : sums[m] * (1.f - s[m]));
+  }
 }
 
 static int route_problem(const char* name, int64_t T, int32_t E, int32_t k, int32_t score, int32_t norm, int32_t dtype) {
@@ -360,6 +619,8 @@ template <typename T, int PER, int W> static void launch(const Args& a, cudaStre
 }
 
 template <typename T> static int dispatch(Args a, cudaStream_t s) {
+  a.id_bits = 1;
+  while ((1 << a.id_bits) < a.E) ++a.id_bits;
   // the fewest lanes per token that keep a group on whole lanes and 16 experts a lane
   int W = 8;
   for (;; W *= 2) {
@@ -369,6 +630,12 @@ template <typename T> static int dispatch(Args a, cudaStream_t s) {
     a.per = (a.gs + (1 << a.shift) - 1) >> a.shift;
     if (a.per <= 16 || W == 32) break;
   }
+  a.shift32 = 0;
+  while ((2 << a.shift32) * a.G <= 32) ++a.shift32;
+  a.per32 = (a.gs + (1 << a.shift32) - 1) >> a.shift32;  // <= 8 where W < 32: 16 experts a lane, 2 or 4 times the lanes
+  const bool vec = a.E % 4 == 0 && a.gs % 4 == 0 && a.per % 4 == 0;
+  a.vec = vec && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
+  a.vec_bias = vec && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
   if (W == 8) a.per <= 8 ? launch<T, 8, 8>(a, s) : launch<T, 16, 8>(a, s);
   else if (W == 16) a.per <= 8 ? launch<T, 8, 16>(a, s) : launch<T, 16, 16>(a, s);
   else if (a.per <= 8) launch<T, 8, 32>(a, s);
@@ -378,15 +645,21 @@ template <typename T> static int dispatch(Args a, cudaStream_t s) {
   return check_launch("route_groups");
 }
 
+template <typename T, int PER, int W>
+static void backward(const float* gw, const void* logits, const int64_t* idx, int64_t tokens, int E, int k, int score,
+                     int norm, float scale, void* out, cudaStream_t s) {
+  const int vec = E % 4 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  route_groups_backward_kernel<T, PER, W><<<(unsigned)((tokens * W + 255) / 256), 256, 0, s>>>(
+      gw, static_cast<const T*>(logits), idx, tokens, E, k, score, norm, vec, scale, static_cast<T*>(out));
+}
+
 template <typename T>
 static void launch_backward(const float* gw, const void* logits, const int64_t* idx, int64_t tokens, int E, int k,
                             int score, int norm, float scale, void* out, cudaStream_t s) {
-  const unsigned grid = (unsigned)((tokens + 7) / 8);
-  const T* l = static_cast<const T*>(logits);
-  T* o = static_cast<T*>(out);
-  if (E <= 128) route_groups_backward_kernel<T, 4><<<grid, 256, 0, s>>>(gw, l, idx, tokens, E, k, score, norm, scale, o);
-  else if (E <= 256) route_groups_backward_kernel<T, 8><<<grid, 256, 0, s>>>(gw, l, idx, tokens, E, k, score, norm, scale, o);
-  else route_groups_backward_kernel<T, 32><<<grid, 256, 0, s>>>(gw, l, idx, tokens, E, k, score, norm, scale, o);
+  if (E <= 64) backward<T, 8, 8>(gw, logits, idx, tokens, E, k, score, norm, scale, out, s);
+  else if (E <= 128) backward<T, 16, 8>(gw, logits, idx, tokens, E, k, score, norm, scale, out, s);
+  else if (E <= 256) backward<T, 16, 16>(gw, logits, idx, tokens, E, k, score, norm, scale, out, s);
+  else backward<T, 32, 32>(gw, logits, idx, tokens, E, k, score, norm, scale, out, s);
 }
 
 }  // namespace rg

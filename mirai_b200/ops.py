@@ -36,6 +36,18 @@ def _cuda(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> torch
     return t.contiguous()
 
 
+def _run(device: torch.device, name: str, *args) -> None:
+    """``name`` on ``device``'s current stream, with that device current.  Pointers go
+    as plain integers (None: null); the small calls are paced by their host time, so
+    this path looks up the stream and the device without building objects."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    with torch.cuda.device(index):
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def device_status() -> tuple[int, int]:
     """Synchronise the current stream and return (and clear) the device error word."""
     return _lib.device_status(torch.cuda.current_stream().cuda_stream)
@@ -127,11 +139,12 @@ def route_groups(logits: torch.Tensor, top_k: int, *, num_groups: int = 1, top_g
     if bias is not None and tuple(bias.shape) != (E,):
         raise ValueError(f"choice_bias of shape {tuple(bias.shape)} for {E} experts")
     _same_device(logits.device, choice_bias=bias)
-    idx = torch.empty((T, max(int(top_k), 0)), dtype=torch.int64, device=logits.device)
-    w = torch.empty((T, max(int(top_k), 0)), dtype=torch.float32, device=logits.device)
-    with torch.cuda.device(logits.device):
-        _lib.call("mirai_route_groups", _ptr(logits), _DTYPE_CODES[logits.dtype], T, E, top_k, num_groups, top_groups,
-                  GROUP_SCORES[group_score], score, _ptr(bias), mode, float(route_scale), _ptr(idx), _ptr(w), _stream())
+    slots = max(int(top_k), 0)
+    idx = torch.empty((T, slots), dtype=torch.int64, device=logits.device)
+    w = torch.empty((T, slots), dtype=torch.float32, device=logits.device)
+    _run(logits.device, "mirai_route_groups", logits.data_ptr(), _DTYPE_CODES[logits.dtype], T, E, top_k, num_groups,
+         top_groups, GROUP_SCORES[group_score], score, None if bias is None else bias.data_ptr(), mode, route_scale,
+         idx.data_ptr(), w.data_ptr())
     return idx, w
 
 
@@ -149,9 +162,8 @@ def route_groups_backward(grad_weights: torch.Tensor, logits: torch.Tensor, top_
         raise ValueError(f"grad_weights {tuple(gw.shape)} and top_indices {tuple(idx.shape)} for {T} tokens")
     _same_device(logits.device, grad_weights=gw, top_indices=idx)
     grad = torch.empty_like(logits)
-    with torch.cuda.device(logits.device):
-        _lib.call("mirai_route_groups_backward", _ptr(gw), _ptr(logits), _DTYPE_CODES[logits.dtype], _ptr(idx), T, E,
-                  idx.shape[1], score, mode, float(route_scale), _ptr(grad), _stream())
+    _run(logits.device, "mirai_route_groups_backward", gw.data_ptr(), logits.data_ptr(), _DTYPE_CODES[logits.dtype],
+         idx.data_ptr(), T, E, idx.shape[1], score, mode, route_scale, grad.data_ptr())
     return grad
 
 
@@ -354,7 +366,7 @@ _MXFP4_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 3}
 
 def _same_device(device: torch.device, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != device:
+        if t is not None and t.device != device:  # (a tensor or an Mxfp4Rows)
             raise ValueError(f"{name} is on {t.device}, the call runs on {device}")
 
 
@@ -394,18 +406,22 @@ class Mxfp4Tensor:
     (``mxfp4_scale_tiles`` makes them of a checkpoint's [E, out, in/32])."""
 
     def __init__(self, packed: torch.Tensor, scale: torch.Tensor):
-        self.packed = _aligned(_cuda(packed, "packed", torch.uint8))
-        self.scale = _aligned(_cuda(scale, "scale", torch.uint8))
-        if self.packed.ndim != 3 or self.packed.shape[2] % (MXFP4_BLOCK // 2) or 0 in self.packed.shape:
-            raise ValueError(f"MXFP4 codes must be [E, out, in/2] with in % 32 == 0, got {tuple(self.packed.shape)}")
-        E, out_f, half = self.packed.shape
+        packed = _aligned(_cuda(packed, "packed", torch.uint8))
+        scale = _aligned(_cuda(scale, "scale", torch.uint8))
+        if packed.ndim != 3 or packed.shape[2] % (MXFP4_BLOCK // 2) or 0 in packed.shape:
+            raise ValueError(f"MXFP4 codes must be [E, out, in/2] with in % 32 == 0, got {tuple(packed.shape)}")
+        E, out_f, half = packed.shape
         want = (E, *_tiles(out_f, 2 * half), 512)
-        if tuple(self.scale.shape) != want:
-            raise ValueError(f"MXFP4 scale tiles of shape {tuple(self.scale.shape)}: {E} x {out_f} x {2 * half} needs "
-                             f"{want}")
-        _same_device(self.packed.device, scale=self.scale)
-        self.shape = (E, out_f, 2 * half)
-        self._struct = _lib.Mxfp4Weight(self.packed.data_ptr(), self.scale.data_ptr())
+        if tuple(scale.shape) != want:
+            raise ValueError(f"MXFP4 scale tiles of shape {tuple(scale.shape)}: {E} x {out_f} x {2 * half} needs {want}")
+        _same_device(packed.device, scale=scale)
+        self._bind(packed, scale)
+
+    def _bind(self, packed: torch.Tensor, scale: torch.Tensor) -> "Mxfp4Tensor":
+        self.packed, self.scale, self.device = packed, scale, packed.device
+        self.shape = (packed.shape[0], packed.shape[1], 2 * packed.shape[2])
+        self._struct = _lib.Mxfp4Weight(packed.data_ptr(), scale.data_ptr())
+        return self
 
     def struct(self) -> _lib.Mxfp4Weight:
         return self._struct
@@ -436,14 +452,17 @@ class Mxfp4Rows:
 
     @staticmethod
     def scale_bytes(rows: int, width: int, segments: int) -> int:
-        return int(_lib.load().mirai_mxfp4_rows_scale_bytes(rows, segments, width))
+        """mirai_mxfp4_rows_scale_bytes: every segment can end inside a row tile."""
+        return (rows // 128 + min(rows, segments)) * _tiles(0, width)[1] * 512
 
     @classmethod
     def empty(cls, rows: int, width: int, segments: int, device) -> "Mxfp4Rows":
+        r = cls.__new__(cls)
         kt = _tiles(0, width)[1]
-        tiles = cls.scale_bytes(rows, width, segments) // (512 * kt)
-        return cls(torch.empty((rows, width // 2), dtype=torch.uint8, device=device),
-                   torch.empty((tiles, kt, 512), dtype=torch.uint8, device=device), segments)
+        r.packed = torch.empty((rows, width // 2), dtype=torch.uint8, device=device)
+        r.scale = torch.empty((rows // 128 + min(rows, segments), kt, 512), dtype=torch.uint8, device=device)
+        r.segments, r.shape, r.device = segments, (rows, width), device
+        return r
 
 
 def mxfp4_quantize(weight: torch.Tensor) -> Mxfp4Tensor:
@@ -461,10 +480,9 @@ def mxfp4_quantize(weight: torch.Tensor) -> Mxfp4Tensor:
     # rows past `out` in the last tile are zero bytes too
     make = torch.empty if out_f % 128 == 0 else torch.zeros
     scale = make((E, *_tiles(out_f, in_f), 512), dtype=torch.uint8, device=w.device)
-    with torch.cuda.device(w.device):
-        _lib.call("mirai_mxfp4_quantize", _ptr(w), _MXFP4_DTYPES[w.dtype], E, out_f, in_f, _ptr(packed), _ptr(scale),
-                  _stream())
-    return Mxfp4Tensor(packed, scale)
+    _run(w.device, "mirai_mxfp4_quantize", w.data_ptr(), _MXFP4_DTYPES[w.dtype], E, out_f, in_f, packed.data_ptr(),
+         scale.data_ptr())
+    return Mxfp4Tensor.__new__(Mxfp4Tensor)._bind(packed, scale)
 
 
 def mxfp4_dequantize(w: Mxfp4Tensor, out: torch.Tensor | None = None,
@@ -476,15 +494,14 @@ def mxfp4_dequantize(w: Mxfp4Tensor, out: torch.Tensor | None = None,
     if out is None:
         if out_dtype not in _MXFP4_DTYPES:
             raise TypeError(f"mxfp4_dequantize writes bf16, fp32 or fp16, not {out_dtype}")
-        out = torch.empty(w.shape, dtype=out_dtype, device=w.packed.device)
-    if out.dtype not in _MXFP4_DTYPES or tuple(out.shape) != w.shape or not out.is_contiguous() or out.data_ptr() % 32:
+        out = torch.empty(w.shape, dtype=out_dtype, device=w.device)
+    elif out.dtype not in _MXFP4_DTYPES or tuple(out.shape) != w.shape or not out.is_contiguous() or out.data_ptr() % 32:
         raise ValueError(f"out must be a contiguous, 32-byte aligned {w.shape} tensor of bf16, fp32 or fp16, got "
                          f"{out.dtype} {tuple(out.shape)}")
-    _same_device(w.packed.device, out=out)
+    _same_device(w.device, out=out)
     E, out_f, in_f = w.shape
-    with torch.cuda.device(out.device):
-        _lib.call("mirai_mxfp4_dequantize", _ptr(w.packed), _ptr(w.scale), E, out_f, in_f, _ptr(out),
-                  _MXFP4_DTYPES[out.dtype], _stream())
+    _run(w.device, "mirai_mxfp4_dequantize", w.packed.data_ptr(), w.scale.data_ptr(), E, out_f, in_f, out.data_ptr(),
+         _MXFP4_DTYPES[out.dtype])
     return out
 
 
@@ -500,9 +517,8 @@ def mxfp4_quantize_rows(x: torch.Tensor, offsets: torch.Tensor, row_index: torch
     _same_device(x.device, offsets=offsets, row_index=index)
     S = x.shape[0] if index is None else index.numel()
     rows = Mxfp4Rows.empty(S, x.shape[1], offsets.numel(), x.device)
-    with torch.cuda.device(x.device):
-        _lib.call("mirai_mxfp4_quantize_rows", _ptr(x), x.shape[0], _ptr(index), _ptr(offsets), offsets.numel(), S,
-                  x.shape[1], _ptr(rows.packed), _ptr(rows.scale), _stream())
+    _run(x.device, "mirai_mxfp4_quantize_rows", x.data_ptr(), x.shape[0], None if index is None else index.data_ptr(),
+         offsets.data_ptr(), offsets.numel(), S, x.shape[1], rows.packed.data_ptr(), rows.scale.data_ptr())
     return rows
 
 
@@ -533,17 +549,17 @@ def _gateup_mxfp4(x, offsets: torch.Tensor, w1: Mxfp4Tensor, w3: Mxfp4Tensor, *,
     if out_f != inter or offsets.numel() != sources * E:
         raise ValueError(f"keys of {E} experts x {out_f} channels: the call has inter {inter} and {offsets.numel()} "
                          f"segments of {sources} source(s)")
-    device = w1.packed.device
-    _same_device(device, x=x, offsets=offsets, w3=w3.packed)
+    device = w1.device
+    _same_device(device, x=x, offsets=offsets, w3=w3)
     rows = _mxfp4_rows(x, offsets, hidden, "x_sorted")
     S = rows.shape[0]
     h = _mxfp4_output(out, (S, inter), device) if want_h else None
     gu = torch.empty((S, 2 * inter), dtype=torch.bfloat16, device=device) if save_gate_up else None
     hq = Mxfp4Rows.empty(S, inter, offsets.numel(), device) if want_rows else None
-    with torch.cuda.device(device):
-        _lib.call("mirai_moe_gateup_swiglu_mxfp4", _ptr(rows.packed), _ptr(rows.scale), _ptr(offsets), sources, E, S,
-                  hidden, inter, w1.struct(), w3.struct(), _ptr(h), _ptr(gu), _ptr(hq.packed if hq else None),
-                  _ptr(hq.scale if hq else None), _stream())
+    _run(device, "mirai_moe_gateup_swiglu_mxfp4", rows.packed.data_ptr(), rows.scale.data_ptr(), offsets.data_ptr(),
+         sources, E, S, hidden, inter, w1.struct(), w3.struct(), None if h is None else h.data_ptr(),
+         None if gu is None else gu.data_ptr(), None if hq is None else hq.packed.data_ptr(),
+         None if hq is None else hq.scale.data_ptr())
     return h, gu, hq
 
 
@@ -554,7 +570,7 @@ def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: 
     if out_f != hidden or offsets.numel() != sources * E:
         raise ValueError(f"a key of {E} experts x {out_f} rows: the call has hidden {hidden} and {offsets.numel()} "
                          f"segments of {sources} source(s)")
-    device = w2.packed.device
+    device = w2.device
     _same_device(device, h=h, offsets=offsets, rank_a=rank_a)
     low = rank_b = None
     if lora is not None:
@@ -570,9 +586,9 @@ def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: 
     rows = _mxfp4_rows(h, offsets, inter, "h")
     S = rows.shape[0]
     y = _mxfp4_output(out, (S, hidden), device)
-    with torch.cuda.device(device):
-        _lib.call("mirai_moe_down_mxfp4", _ptr(rows.packed), _ptr(rows.scale), _ptr(offsets), sources, E, S, inter, hidden,
-                  w2.struct(), _ptr(low), _ptr(rank_b), _ptr(y), _stream())
+    _run(device, "mirai_moe_down_mxfp4", rows.packed.data_ptr(), rows.scale.data_ptr(), offsets.data_ptr(), sources, E, S,
+         inter, hidden, w2.struct(), None if low is None else low.data_ptr(),
+         None if rank_b is None else rank_b.data_ptr(), y.data_ptr())
     return y
 
 
