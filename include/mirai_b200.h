@@ -601,6 +601,17 @@ int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const 
                          const mirai_mxfp4_weight* w2, const void* rank_a, const void* rank_b, void* y,
                          mirai_stream_t stream);
 
+/* The same products for at most MIRAI_MXFP4_FEW_ROWS rows given in bf16 (32-byte aligned), of
+ * at most 4096 elements: quantised in the kernel, which reads the weights of the experts that
+ * have rows and little else (a generation step).  gate_up may be NULL. */
+enum { MIRAI_MXFP4_FEW_ROWS = 1024 };
+int mirai_moe_gateup_swiglu_mxfp4_few(const void* x, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                                      int64_t num_rows, int32_t hidden, int32_t inter, const mirai_mxfp4_weight* w1,
+                                      const mirai_mxfp4_weight* w3, void* h, void* gate_up, mirai_stream_t stream);
+int mirai_moe_down_mxfp4_few(const void* h, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                             int64_t num_rows, int32_t inter, int32_t hidden, const mirai_mxfp4_weight* w2, void* y,
+                             mirai_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -182,6 +182,11 @@ SIGNATURES = {
     "mirai_moe_gateup_swiglu_mxfp4": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
                                                      ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight), c_vp,
                                                      c_vp, c_vp, c_vp, c_vp]),
+    "mirai_moe_gateup_swiglu_mxfp4_few": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
+                                                         ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight),
+                                                         c_vp, c_vp, c_vp]),
+    "mirai_moe_down_mxfp4_few": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
+                                                ctypes.POINTER(Mxfp4Weight), c_vp, c_vp]),
     "mirai_moe_down_mxfp4": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
                                             ctypes.POINTER(Mxfp4Weight), c_vp, c_vp, c_vp, c_vp]),
 }

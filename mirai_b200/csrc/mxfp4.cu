@@ -193,7 +193,14 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint8_t* tiles = scale + (int64_t)blk * kt * 512;
-  for (int r = strip * kStrip + warp; r < min(b.rows, (strip + 1) * kStrip); r += 8) {
+  // a matrix's scale tiles are written whole: zero bytes past its last row
+  const int last = ROWS ? b.rows : kBlockRows;
+  for (int r = strip * kStrip + warp; r < min(last, (strip + 1) * kStrip); r += 8) {
+    if (!ROWS && r >= b.rows) {
+      for (int kw = lane; kw < kt; kw += 32)
+        *reinterpret_cast<uint32_t*>(tiles + (int64_t)kw * 512 + (r & 31) * 16 + (r >> 5) * 4) = 0u;
+      continue;
+    }
     const int64_t dst = b.row0 + r;
     int64_t src = dst;
     bool ok = true;
@@ -971,6 +978,347 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // ----------------------------------------------------------------------------
+// The same products for few rows (a generation step): the weights are read once
+// and nothing else counts, so the roles of the operands are exchanged -- 128
+// channels of the weights are the MMA's M, up to 32 rows its N -- and a tile is
+// one SM's: 128 channels of gate and the same 128 of up (DOWN: 128 outputs) of one
+// segment.  The rows come in bf16 and are quantised here, into the swizzled operand,
+// while the weights are on their way: one launch instead of two, no row buffer.
+// A lane of the accumulator is a channel, a column a row, so a warp stores 64
+// contiguous bytes of h per row.
+//
+// Warps: 0 TMA producer, 1 MMA issuer, 4..11 quantise the rows, 4..7 then move scales to
+// TMEM and are the epilogue.
+constexpr int FEW_ROWS = 32;    // rows of a tile
+constexpr int FEW_STAGES = 6;   // most weight stages (and TMEM scale slots)
+constexpr int FEW_QUANT = 8;    // quantising warps
+constexpr int FEW_THREADS = 32 * (4 + FEW_QUANT);
+constexpr int FEW_MAX_K = 4096;
+constexpr uint32_t FEW_SF_COL = 64;
+constexpr uint32_t FEW_COLS = 256;
+
+struct FewParams {
+  const __nv_bfloat16* x;  // [S, K]
+  const int32_t* offsets;
+  int segs, experts;
+  int64_t S;
+  int K, N;
+  int n_tiles, w_blocks, stages;
+  __nv_bfloat16* out;      // [S, N]
+  __nv_bfloat16* gate_up;  // GATEUP: optional [S, 2N]
+};
+
+struct alignas(16) FewSmem {
+  uint64_t full[FEW_STAGES];     // the producer (bytes of codes) and four scale warps
+  uint64_t empty[FEW_STAGES];
+  uint64_t sf_full[FEW_STAGES];  // bytes of scales
+  uint64_t rows_ready;           // quantising warps
+  uint64_t tfull, tempty;
+  uint32_t tmem_base;
+  int abort_flag;
+  // followed by the segments' first rows and tile prefixes [segs + 1] each
+};
+template <int MODE> constexpr uint32_t few_stage_bytes() { return (MODE == GATEUP ? 2 : 1) * (A_BYTES + 1024); }
+template <int MODE> static size_t few_smem_bytes(int stages, int K, int segs) {
+  const int kbs = (K + BKE - 1) / BKE;
+  return 1024 + (size_t)stages * few_stage_bytes<MODE>() + (size_t)kbs * (FEW_ROWS * 128 + 256) + sizeof(FewSmem) +
+         ((size_t)2 * (segs + 1) * sizeof(int) + 15) / 16 * 16;
+}
+
+__device__ __forceinline__ void umma_mxf4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %7};\n\t"
+      "mov.b64 db, {%2, %7};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(DESC_HI)
+      : "memory");
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w0, const __grid_constant__ CUtensorMap tmap_w1,
+                    const __grid_constant__ CUtensorMap tmap_s0, const __grid_constant__ CUtensorMap tmap_s1,
+                    const __grid_constant__ FewParams p) {
+  constexpr int KEYS = MODE == GATEUP ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int num_kb = (p.K + BKE - 1) / BKE;
+  uint8_t* sW = base;                                            // per stage: KEYS x 16 KB of codes
+  uint8_t* sX = sW + p.stages * KEYS * A_BYTES;                  // per k-block: 32 rows x 128 bytes (swizzled)
+  uint8_t* sSF = sX + num_kb * FEW_ROWS * 128;                   // per stage: KEYS x 1 KB of weight scales
+  uint32_t* sXS = reinterpret_cast<uint32_t*>(sSF + p.stages * KEYS * 1024);  // per K tile: 32 words of row scales
+  FewSmem& sm = *reinterpret_cast<FewSmem*>(reinterpret_cast<uint8_t*>(sXS) + num_kb * 256);
+  int* row_start = reinterpret_cast<int*>(&sm + 1);
+  int* prefix = row_start + p.segs + 1;  // (first the segments' rows, then tiles before each)
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int g = threadIdx.x; g < p.segs; g += FEW_THREADS) {
+    int begin;
+    prefix[g] = segment_rows(p.offsets, g, p.S, begin, 720 + MODE);
+    row_start[g] = begin;
+  }
+  if (warp == 1) {
+    if (lane == 0) {
+      for (int i = 0; i < FEW_STAGES; ++i) {
+        mbar_init(&sm.full[i], 1 + 4);
+        mbar_init(&sm.empty[i], 1);
+        mbar_init(&sm.sf_full[i], 1);
+      }
+      mbar_init(&sm.rows_ready, FEW_QUANT);
+      mbar_init(&sm.tfull, 1);
+      mbar_init(&sm.tempty, 4);
+      sm.abort_flag = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(&sm.tmem_base, FEW_COLS);
+    tmem_relinquish();
+  }
+  if (warp == 2 && lane == 0) {
+    prefetch_tmap(&tmap_w0);
+    prefetch_tmap(&tmap_s0);
+    if (KEYS == 2) {
+      prefetch_tmap(&tmap_w1);
+      prefetch_tmap(&tmap_s1);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {  // tiles (32 rows) before each segment
+    int carry = 0;
+    for (int g0 = 0; g0 < p.segs; g0 += 32) {
+      const int g = g0 + lane;
+      const int rows = g < p.segs ? prefix[g] : 0;
+      const int n = (rows + FEW_ROWS - 1) / FEW_ROWS;
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (g < p.segs) {
+        prefix[g] = carry + incl - n;
+        if (g == p.segs - 1) row_start[p.segs] = row_start[g] + rows;
+      }
+      carry += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) prefix[p.segs] = carry;
+  }
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem = sm.tmem_base;
+  const int tiles = prefix[p.segs] * p.n_tiles;
+  volatile int* abort_flag = &sm.abort_flag;
+  struct Tile {
+    int row, rows, expert, n;
+  };
+  auto decode = [&](int t) {
+    const int mt = t / p.n_tiles;
+    int lo = 0, hi = p.segs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= mt) lo = mid;
+      else hi = mid;
+    }
+    const int m = mt - prefix[lo], row = row_start[lo] + m * FEW_ROWS;
+    return Tile{row, min(FEW_ROWS, row_start[lo + 1] - row), lo % p.experts, t - mt * p.n_tiles};
+  };
+
+  if (warp == 0 && lane == 0) {
+    // ======================= TMA producer =======================
+    Ring r;
+    for (int t = (int)blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x) {
+      const Tile tl = decode(t);
+      const int wrow = tl.expert * p.N + tl.n * BM, wblk = tl.expert * p.w_blocks + tl.n;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(&sm.empty[r.i], r.phase ^ 1, 60)) {
+          *abort_flag = 1;
+          break;
+        }
+        uint8_t* w = sW + r.i * KEYS * A_BYTES;
+        uint8_t* sf = sSF + r.i * KEYS * 1024;
+        mbar_arrive_expect_tx(&sm.full[r.i], KEYS * A_BYTES);
+        tma_load_2d(w, &tmap_w0, kb * 128, wrow, &sm.full[r.i]);
+        if (KEYS == 2) tma_load_2d(w + A_BYTES, &tmap_w1, kb * 128, wrow, &sm.full[r.i]);
+        mbar_arrive_expect_tx(&sm.sf_full[r.i], KEYS * 1024);
+        tma_load_2d(sf, &tmap_s0, kb * 256, wblk, &sm.sf_full[r.i]);
+        if (KEYS == 2) tma_load_2d(sf + 1024, &tmap_s1, kb * 256, wblk, &sm.sf_full[r.i]);
+        r.next(p.stages);
+      }
+    }
+  } else if (warp == 1) {
+    // ======================= MMA issuer =======================
+    const bool issue = elect_one();
+    constexpr uint32_t id0 = idesc_mxf4(BM, FEW_ROWS, 0), id2 = idesc_mxf4(BM, FEW_ROWS, 2);
+    const uint32_t w_lo0 = desc_lo(smem_u32(sW)), x_lo0 = desc_lo(smem_u32(sX));
+    Ring r;
+    uint32_t done = 0;
+    bool ok = true;
+    for (int t = (int)blockIdx.x; t < tiles && ok && !*abort_flag; t += gridDim.x, ++done) {
+      if (!mbar_wait(&sm.rows_ready, done & 1, 61) || (done > 0 && !mbar_wait(&sm.tempty, (done - 1) & 1, 62))) ok = false;
+      for (int kb = 0; kb < num_kb && ok; ++kb) {
+        if (!mbar_wait(&sm.full[r.i], r.phase, 63)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t w = w_lo0 + r.i * (KEYS * A_BYTES >> 4), x = x_lo0 + kb * (FEW_ROWS * 128 >> 4);
+        const uint32_t sf = tmem + FEW_SF_COL + r.i * 32;
+        const int steps = min(4, (p.K - kb * BKE + 63) / 64);
+        if (issue) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k >= steps) break;
+            const uint32_t id = k & 1 ? id2 : id0;
+            umma_mxf4(tmem, w + 2 * k, x + 2 * k, id, sf + 4 * (k >> 1), sf + 16 + 4 * (k >> 1), (kb | k) != 0);
+            if (KEYS == 2)
+              umma_mxf4(tmem + FEW_ROWS, w + (A_BYTES >> 4) + 2 * k, x + 2 * k, id, sf + 8 + 4 * (k >> 1),
+                        sf + 16 + 4 * (k >> 1), (kb | k) != 0);
+          }
+          umma_commit(&sm.empty[r.i]);
+        }
+        __syncwarp();
+        r.next(p.stages);
+      }
+      if (ok && issue) umma_commit(&sm.tfull);
+      __syncwarp();
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    // the last commits have arrived before the CTA frees its barriers and TMEM
+    for (int i = 0; i < p.stages; ++i) {
+      if (!mbar_wait(&sm.empty[r.i], r.phase ^ 1, 64)) break;
+      r.next(p.stages);
+    }
+  } else if (warp >= 4) {
+    // ======================= rows, scales, epilogue =======================
+    const int q = warp & 3;
+    Ring r;
+    uint32_t done = 0;
+    for (int t = (int)blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x, ++done) {
+      const Tile tl = decode(t);
+      // the previous tile's MMAs have read the rows
+      if (done > 0 && !mbar_wait(&sm.tfull, (done - 1) & 1, 65)) {
+        *abort_flag = 1;
+        break;
+      }
+      for (int i = warp - 4; i < tl.rows; i += FEW_QUANT) {
+        const __nv_bfloat16* row = p.x + (int64_t)(tl.row + i) * p.K;
+        for (int b = 0; b < num_kb * BKE; b += kStep * 4) {
+          Raw16<__nv_bfloat16> raw[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = b + j * kStep + lane * 16;
+            if (k < p.K) load16(row + k, raw[j]);
+            else raw[j] = Raw16<__nv_bfloat16>{};
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = b + j * kStep + lane * 16;
+            if (b + j * kStep >= num_kb * BKE) break;  // warp-uniform
+            uint32_t m = amax16(raw[j]);
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            const uint32_t byte = scale_byte(m);
+            const float inv = inv_scale(byte == 255u ? 254u : byte);
+            uint32_t codes[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float v[8];
+              unpack8(raw[j], h, v);
+#pragma unroll
+              for (int z = 0; z < 8; ++z) v[z] *= inv;
+              codes[h] = byte == 255u ? 0u : e2m1x8(v);
+            }
+            uint32_t w = byte << (8 * ((lane >> 1) & 3));
+            w |= __shfl_xor_sync(0xffffffffu, w, 2);
+            w |= __shfl_xor_sync(0xffffffffu, w, 4);
+            if (k < num_kb * BKE) {  // 8 bytes of a 128-byte row, 16-byte chunks swizzled by the row
+              const uint32_t chunk = (uint32_t)((k % BKE) / 32) ^ (uint32_t)(i & 7);
+              *reinterpret_cast<uint2*>(sX + (k / BKE) * (FEW_ROWS * 128) + i * 128 + chunk * 16 + (lane & 1) * 8) =
+                  make_uint2(codes[0], codes[1]);
+              if ((lane & 7) == 0) sXS[(k / 128) * 32 + i] = w;
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.rows_ready);
+      if (warp >= 8) continue;
+      // every quantising warp's scale words are read here
+      if (!mbar_wait(&sm.rows_ready, done & 1, 68)) {
+        *abort_flag = 1;
+        break;
+      }
+      const uint32_t quarter = (uint32_t)(q * 32) << 16;
+      bool ok = true;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(&sm.sf_full[r.i], r.phase, 66)) {
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t src = smem_u32(sSF + r.i * KEYS * 1024) + lane * 16u;
+        const uint32_t dst = tmem + FEW_SF_COL + r.i * 32 + quarter;
+        tmem_st_x8(dst, lds128(src), lds128(src + 512));
+        if (KEYS == 2) tmem_st_x8(dst + 8, lds128(src + 1024), lds128(src + 1536));
+        tmem_st_x8(dst + 16, make_uint4(sXS[2 * kb * 32 + lane], 0, 0, 0), make_uint4(sXS[(2 * kb + 1) * 32 + lane], 0, 0, 0));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.full[r.i]);
+        r.next(p.stages);
+      }
+      if (!ok) break;
+      if (!mbar_wait(&sm.tfull, done & 1, 67)) {
+        *abort_flag = 1;
+        break;
+      }
+      __syncwarp();
+      tc_fence_after();
+      uint32_t g[32], up[32];
+      tmem_ld_32x32b_x32(tmem + quarter, g);
+      if (KEYS == 2) tmem_ld_32x32b_x32(tmem + FEW_ROWS + quarter, up);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.tempty);
+      const int ch = tl.n * BM + q * 32 + lane;
+      if (ch < p.N) {
+        __nv_bfloat16* dst = p.out + (int64_t)tl.row * p.N + ch;
+#pragma unroll
+        for (int i = 0; i < FEW_ROWS; ++i) {
+          if (i >= tl.rows) break;
+          const float gv = __uint_as_float(g[i]);
+          if (MODE == GATEUP) {
+            const float uv = __uint_as_float(up[i]);
+            dst[(int64_t)i * p.N] = __float2bfloat16_rn(silu(gv) * uv);
+            if (p.gate_up) {
+              __nv_bfloat16* gu = p.gate_up + (int64_t)(tl.row + i) * 2 * p.N + ch;
+              gu[0] = __float2bfloat16_rn(gv);
+              gu[p.N] = __float2bfloat16_rn(uv);
+            }
+          } else {
+            dst[(int64_t)i * p.N] = __float2bfloat16_rn(gv);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, FEW_COLS);
+  }
+}
+
+// ----------------------------------------------------------------------------
 // host side
 
 static bool misaligned(const void* p, unsigned a = 16) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
@@ -1146,6 +1494,65 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   return check_launch(name);
 }
 
+// Few rows in bf16 (see few_rows_kernel).
+template <int MODE>
+static int few_product(const char* name, const void* x, const int32_t* offsets, int32_t nsrc, int32_t experts, int64_t S,
+                       int32_t K, int32_t N, const mirai_mxfp4_weight* w0, const mirai_mxfp4_weight* w1, void* out,
+                       void* gate_up, mirai_stream_t stream) {
+  if (nsrc <= 0 || experts <= 0 || (int64_t)nsrc * experts > kMaxSegs)
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: %d sources x %d experts outside 1..%d segments", name, nsrc, experts,
+                     kMaxSegs);
+  if (S < 0 || K <= 0 || N <= 0)
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: bad sizes (S=%lld, K=%d, N=%d)", name, (long long)S, K, N);
+  if (K % 32 || N % 32 || K > FEW_MAX_K || S > MIRAI_MXFP4_FEW_ROWS)
+    return set_error(MIRAI_ERR_UNSUPPORTED, "%s: needs K %% 32 == 0 up to %d, N %% 32 == 0 and at most %d rows (S=%lld, "
+                     "K=%d, N=%d)", name, FEW_MAX_K, MIRAI_MXFP4_FEW_ROWS, (long long)S, K, N);
+  if ((int64_t)experts * N >= (int64_t)1 << 31)
+    return set_error(MIRAI_ERR_UNSUPPORTED, "%s: more than 2^31 weight rows", name);
+  if (S == 0) return MIRAI_OK;
+  if (!x || !offsets || !out || !w0 || !w0->packed || !w0->scale || (w1 && (!w1->packed || !w1->scale)))
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: null operand", name);
+  if (misaligned(x, 32)) return set_error(MIRAI_ERR_INVALID_ARG, "%s: rows not 32-byte aligned", name);
+  const int kt = (int)ceil_div(K, 128);
+  FewParams p = {};
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.offsets = offsets;
+  p.segs = nsrc * experts;
+  p.experts = experts;
+  p.S = S;
+  p.K = K;
+  p.N = N;
+  p.n_tiles = (int)ceil_div(N, BM);
+  p.w_blocks = p.n_tiles;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.gate_up = static_cast<__nv_bfloat16*>(gate_up);
+  p.stages = FEW_STAGES;
+  while (few_smem_bytes<MODE>(p.stages, K, p.segs) > kSmemLimit) --p.stages;
+  CUtensorMap t0, t1, s0, s1;
+  int rc = code_map(t0, w0->packed, (int64_t)experts * N, K);
+  if (!rc) rc = scale_map(s0, w0->scale, (int64_t)experts * p.w_blocks, kt);
+  if (!rc) rc = w1 ? code_map(t1, w1->packed, (int64_t)experts * N, K) : (t1 = t0, MIRAI_OK);
+  if (!rc) rc = w1 ? scale_map(s1, w1->scale, (int64_t)experts * p.w_blocks, kt) : (s1 = s0, MIRAI_OK);
+  if (rc) return rc;
+  static std::atomic<bool> ready[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
+    return set_error(MIRAI_ERR_CUDA, "%s: no current device", name);
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(few_rows_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimit);
+    if (e != cudaSuccess) return set_error(MIRAI_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  const int limit = gemm_sm_limit();
+  int64_t grid = (S / FEW_ROWS + (p.segs < S ? p.segs : S)) * p.n_tiles;
+  const int sms = (limit > 0 && limit < sm_count()) ? limit : sm_count();
+  if (grid > sms) grid = sms;
+  few_rows_kernel<MODE><<<(unsigned)grid, FEW_THREADS, few_smem_bytes<MODE>(p.stages, K, p.segs),
+                          reinterpret_cast<cudaStream_t>(stream)>>>(t0, t1, s0, s1, p);
+  return check_launch(name);
+}
+
 // Grid of the quantise / read-back kernels, or -1 (with the error set).
 static int64_t strips(const char* name, int64_t blocks) {
   const int64_t g = blocks * (kBlockRows / kStrip);
@@ -1251,6 +1658,21 @@ int mirai_moe_gateup_swiglu_mxfp4(const uint8_t* x_packed, const uint8_t* x_scal
   if (!w3) return set_error(MIRAI_ERR_INVALID_ARG, "gateup_swiglu_mxfp4: null operand");
   return mx::product<mx::GATEUP>("gateup_swiglu_mxfp4", {x_packed, x_scale}, offsets, num_sources, num_experts, num_rows,
                                  hidden, inter, w1, w3, nullptr, nullptr, h, gate_up, h_packed, h_scale, stream);
+}
+
+int mirai_moe_gateup_swiglu_mxfp4_few(const void* x, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                                      int64_t num_rows, int32_t hidden, int32_t inter, const mirai_mxfp4_weight* w1,
+                                      const mirai_mxfp4_weight* w3, void* h, void* gate_up, mirai_stream_t stream) {
+  if (!w3) return set_error(MIRAI_ERR_INVALID_ARG, "gateup_swiglu_mxfp4_few: null operand");
+  return mx::few_product<mx::GATEUP>("gateup_swiglu_mxfp4_few", x, offsets, num_sources, num_experts, num_rows, hidden,
+                                     inter, w1, w3, h, gate_up, stream);
+}
+
+int mirai_moe_down_mxfp4_few(const void* h, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                             int64_t num_rows, int32_t inter, int32_t hidden, const mirai_mxfp4_weight* w2, void* y,
+                             mirai_stream_t stream) {
+  return mx::few_product<mx::DOWN>("down_mxfp4_few", h, offsets, num_sources, num_experts, num_rows, inter, hidden, w2,
+                                   nullptr, y, nullptr, stream);
 }
 
 int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const int32_t* offsets, int32_t num_sources,

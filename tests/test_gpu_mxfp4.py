@@ -162,15 +162,25 @@ def test_quantised_rows_match_the_matrix_quantiser(counts, width):
 
 # ----------------------------------------------------------------------------- products
 
+@pytest.fixture(params=["few", "general"])
+def path(request, monkeypatch):
+    """Both kernels of the products, whatever the rule on the rows would pick."""
+    from mirai_b200 import ops
+    monkeypatch.setattr(ops, "MXFP4_FEW_ROWS", 1024 if request.param == "few" else -1)
+    monkeypatch.setattr(ops, "MXFP4_FEW_ROWS_PER_SEGMENT", 0)
+    return request.param
+
+
 CASES = [
     ([1], 32, 32), ([5], 64, 96), ([130], 96, 160), ([3, 0, 7, 0], 160, 64), ([257, 1, 0, 300], 288, 416),
     ([64, 512], 1408, 256), ([1, 1, 1, 1, 1, 1, 1, 1], 2048, 192), ([700, 0, 33], 544, 1056),
     ([0, 0, 0, 1], 256, 128), ([256, 256], 512, 512), ([2000], 320, 288),
+    ([31, 32, 33, 0, 65], 4096, 96),
 ]
 
 
 @pytest.mark.parametrize("counts,K,N", CASES)
-def test_gateup_matches_64_bits(counts, K, N):
+def test_gateup_matches_64_bits(path, counts, K, N):
     dev = _dev()
     from mirai_b200 import ops
     E, S = len(counts), sum(counts)
@@ -192,7 +202,7 @@ def test_gateup_matches_64_bits(counts, K, N):
 
 
 @pytest.mark.parametrize("counts,K,N", CASES)
-def test_down_matches_64_bits(counts, K, N):
+def test_down_matches_64_bits(path, counts, K, N):
     dev = _dev()
     from mirai_b200 import ops
     x, off = rows(sum(counts), K, dev), segments(counts, dev)
@@ -219,7 +229,7 @@ def test_quantised_gateup_feeds_down(counts, K, N):
     ops.check_device()
 
 
-def test_source_major_segments():
+def test_source_major_segments(path):
     """Two sources' segments give what each source alone gives."""
     dev = _dev()
     from mirai_b200 import ops
