@@ -591,7 +591,7 @@ int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_
  * scales of width I), of the bf16-rounded h; gate_up (may be NULL) [S, 2I] bf16 is saved for
  * the backward.  down: y [S, H] = h W2^T; rank_a [S, 64] / rank_b [E*H, 64] bf16 (both or
  * neither) add a LoRA adapter's rank block, as in mirai_moe_down_lora_bf16.  The backward of
- * both multiplies the read-back weights (mirai_moe_down_dx_bf16, mirai_moe_gateup_dx_bf16). */
+ * both multiplies the read-back weights (mirai_moe_down_dx_f32_bf16, mirai_moe_gateup_dx_bf16). */
 int mirai_moe_gateup_swiglu_mxfp4(const uint8_t* x_packed, const uint8_t* x_scale, const int32_t* offsets,
                                   int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
                                   int32_t inter, const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3, void* h,
@@ -600,6 +600,13 @@ int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const 
                          int32_t num_experts, int64_t num_rows, int32_t inter, int32_t hidden,
                          const mirai_mxfp4_weight* w2, const void* rank_a, const void* rank_b, void* y,
                          mirai_stream_t stream);
+
+/* mirai_moe_down_dx_bf16 (rank_a / rank_b NULL) or mirai_moe_down_dx_lora_bf16 over num_sources *
+ * num_experts segments, with the SwiGLU backward formed in fp32 from the accumulator and rounded
+ * once: the gradient of the MXFP4 forward's h, on its read-back w2. */
+int mirai_moe_down_dx_f32_bf16(const void* grad_y, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                               int64_t num_rows, int32_t hidden, int32_t inter, const void* w2, const void* gate_up,
+                               const void* rank_a, const void* rank_b, void* grad_gate_up, mirai_stream_t stream);
 
 /* The same products for at most MIRAI_MXFP4_FEW_ROWS rows given in bf16 (32-byte aligned), of
  * at most 4096 elements: quantised in the kernel, which reads the weights of the experts that

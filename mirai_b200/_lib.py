@@ -185,6 +185,8 @@ SIGNATURES = {
     "mirai_moe_gateup_swiglu_mxfp4_few": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
                                                          ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight),
                                                          c_vp, c_vp, c_vp]),
+    "mirai_moe_down_dx_f32_bf16": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp,
+                                                  c_vp, c_vp]),
     "mirai_moe_down_mxfp4_few": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
                                                 ctypes.POINTER(Mxfp4Weight), c_vp, c_vp]),
     "mirai_moe_down_mxfp4": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,

@@ -86,7 +86,9 @@ template <int MODE> struct MCfg {
 // DXDOWN epilogue): SwiGLU h = silu(g) * u (experts.py:301-317), or MAGI-2's
 // swiglu7 h = g' sigmoid(1.702 g') (u' + 1) with g' = min(g, 7) and
 // u' = clamp(u, -7, 7) (grouped_moe.py:287-335).
-enum Act { ACT_SWIGLU = 0, ACT_SWIGLU7 = 1 };
+// ACT_SWIGLU_F32 (DXDOWN on bf16 weights): SwiGLU's backward in fp32 from the accumulator,
+// rounded once, for the formats whose forward rounds h once (MXFP4).
+enum Act { ACT_SWIGLU = 0, ACT_SWIGLU7 = 1, ACT_SWIGLU_F32 = 2 };
 
 // Per (format, pairing) geometry.
 template <int WF, bool PAIR> struct Cfg {
@@ -837,7 +839,23 @@ __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
           if (valid && col < p.N) {
             uint32_t dg[16], du[16];
             // (the register budget of the NF4 / INT8 epilogue warps keeps them on the per-element form)
-            if (WF != W_BF16 || p.act == ACT_SWIGLU7) {
+            if (WF == W_BF16 && p.act == ACT_SWIGLU_F32) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float dgo[2], duo[2];
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                  const float dh = __uint_as_float(v32[2 * j + hh]);
+                  const float gv = hh ? bf16_hi(gw[j]) : bf16_lo(gw[j]);
+                  const float uv = hh ? bf16_hi(uw[j]) : bf16_lo(uw[j]);
+                  const float sg = __fdividef(1.f, 1.f + __expf(-gv));
+                  duo[hh] = dh * gv * sg;
+                  dgo[hh] = dh * uv * sg * (1.f + gv * (1.f - sg));
+                }
+                dg[j] = pack_bf16x2(dgo[0], dgo[1]);
+                du[j] = pack_bf16x2(duo[0], duo[1]);
+              }
+            } else if (WF != W_BF16 || p.act == ACT_SWIGLU7) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
                 float dgo[2], duo[2];
@@ -1796,6 +1814,15 @@ int mirai_moe_down_lora_int8(const void* h, const int32_t* offsets, int32_t num_
   const RankBlock rb{rank_a, rank_b};
   return run<DOWN>("down_lora_int8", h, offsets, num_experts, num_rows, inter, hidden, y, nullptr, wi(w2), wi(w2),
                    hidden, inter, stream, &rb);
+}
+int mirai_moe_down_dx_f32_bf16(const void* grad_y, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                               int64_t num_rows, int32_t hidden, int32_t inter, const void* w2, const void* gate_up,
+                               const void* rank_a, const void* rank_b, void* grad_gate_up, mirai_stream_t stream) {
+  if (!rank_a != !rank_b) return set_error(MIRAI_ERR_INVALID_ARG, "down_dx_f32_bf16: null rank-block operand");
+  const RankBlock rb{rank_a, rank_b};
+  return run<DXDOWN>("down_dx_f32_bf16", grad_y, offsets, num_experts, num_rows, hidden, inter, grad_gate_up,
+                     const_cast<void*>(gate_up), wb(w2), wb(w2), hidden, inter, stream, rank_a ? &rb : nullptr,
+                     num_sources, false, -1, ACT_SWIGLU_F32);
 }
 int mirai_moe_down_dx_lora_bf16(const void* grad_y, const int32_t* offsets, int32_t num_experts, int64_t num_rows,
                                 int32_t hidden, int32_t inter, const void* w2, const void* gate_up,

@@ -20,12 +20,13 @@ ACTIVATIONS = {"swiglu": 0, "swiglu7": 1}
 COMBINE_BF16_ACCUM = 2
 
 
-def _ptr(t: torch.Tensor | None) -> _lib.c_vp:
-    return _lib.c_vp(0 if t is None else t.data_ptr())
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _stream() -> _lib.c_vp:
-    return _lib.c_vp(torch.cuda.current_stream().cuda_stream)
+def _stream() -> int:
+    """The current device's current stream (cudaStream_t), without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _cuda(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -36,16 +37,18 @@ def _cuda(t: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> torch
     return t.contiguous()
 
 
-def _run(device: torch.device, name: str, *args) -> None:
-    """``name`` on ``device``'s current stream, with that device current.  Pointers go
-    as plain integers (None: null); the small calls are paced by their host time, so
-    this path looks up the stream and the device without building objects."""
+def _run(device: torch.device, name: str, *args, stream: int | None = None) -> None:
+    """``name`` on ``device``'s current stream (or ``stream``), with that device current.
+    Pointers go as plain integers (None: null); the small calls are paced by their host
+    time, so this path looks up the stream and the device without building objects."""
     index = device.index
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(index)
     if index == torch._C._cuda_getDevice():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        _lib.call(name, *args, stream)
         return
     with torch.cuda.device(index):
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        _lib.call(name, *args, stream)
 
 
 def device_status() -> tuple[int, int]:
@@ -887,8 +890,11 @@ def down_dx(grad_y: torch.Tensor, offsets: torch.Tensor, w2, gate_up: torch.Tens
     (+ the LoRA path's input gradient when ``lora``).  ``sources`` > 1:
     source-major segments (an expert owner's rows); there ``gate_up=None``
     returns dh [S, I] itself."""
+    if isinstance(w2, Mxfp4Tensor):
+        return _down_dx_mxfp4(grad_y, offsets, w2, gate_up, inter=inter, out=out, lora=lora, rank_a=rank_a,
+                              sources=sources)
     group = getattr(w2, "group_size", 0)  # block-Hadamard INT8: the rotation group of dh
-    w2 = _as_weight(_dx_weight(w2))
+    w2 = _as_weight(w2)
     gy = _cuda(grad_y, "grad_y", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
     S, H = gy.shape
@@ -918,6 +924,31 @@ def down_dx(grad_y: torch.Tensor, offsets: torch.Tensor, w2, gate_up: torch.Tens
     glow = rank_a if rank_a is not None else lora_project(gy, offsets, lora, forward=False)
     _lib.call(f"mirai_moe_down_dx_lora_{_fmt_suffix(w2)}", _ptr(gy), _ptr(offsets), offsets.numel(), S, H, inter,
               _wptr(w2), _ptr(gu), _ptr(glow), _ptr(lora.a_pad()), _ptr(dgu), _stream())
+    return dgu
+
+
+def _down_dx_mxfp4(grad_y, offsets, w2: Mxfp4Tensor, gate_up, *, inter: int, out, lora, rank_a, sources: int,
+                   dense: torch.Tensor | None = None) -> torch.Tensor:
+    """``down_dx`` on an MXFP4 key: its read-back values (``dense`` when the caller has
+    them), the SwiGLU backward in fp32 as the forward's."""
+    gy = _cuda(grad_y, "grad_y", torch.bfloat16)
+    offsets = _cuda(offsets, "offsets", torch.int32)
+    gu = _cuda(gate_up, "gate_up", torch.bfloat16)  # (no dh alone: the MXFP4 forward saves gate/up)
+    E, hidden, key_inter = w2.shape
+    S = gy.shape[0]
+    if gy.shape != (S, hidden) or key_inter != inter or gu.shape != (S, 2 * inter) or offsets.numel() != sources * E:
+        raise ValueError(f"grad_y {tuple(gy.shape)}, gate_up {tuple(gu.shape)} and {offsets.numel()} segments do not fit "
+                         f"a key {w2.shape} with inter {inter} and {sources} source(s)")
+    _same_device(w2.device, grad_y=gy, offsets=offsets, gate_up=gu, rank_a=rank_a)
+    w = mxfp4_dequantize(w2) if dense is None else dense
+    low = rank_b = None
+    if lora is not None:
+        low = rank_a if rank_a is not None else lora_project(gy, offsets, lora, forward=False, sources=sources)
+        rank_b = lora.a_pad()
+    dgu = _mxfp4_output(out, (S, 2 * inter), w2.device)
+    _run(w2.device, "mirai_moe_down_dx_f32_bf16", gy.data_ptr(), offsets.data_ptr(), sources, E, S, hidden, inter,
+         w.data_ptr(), gu.data_ptr(), None if low is None else low.data_ptr(),
+         None if rank_b is None else rank_b.data_ptr(), dgu.data_ptr())
     return dgu
 
 
@@ -1174,6 +1205,26 @@ def _stage_beside(weights, rows: int, num_experts: int, *, training: bool):
     return tuple(w if o is None else o for w, o in zip(weights, outs)), (lambda: main.wait_event(done))
 
 
+def _read_back_beside(weights):
+    """bf16 values of MXFP4 keys, read back one after the other on a side stream.  Returns
+    (values, join): ``join(n)`` makes the current stream wait for the first n of them.
+    Every value must be joined before it is read or dropped."""
+    device = weights[0].device
+    main = torch.cuda.current_stream(device)
+    side = _side_streams.get(device.index)
+    if side is None:
+        side = _side_streams.setdefault(device.index, torch.cuda.Stream(device=device))
+    outs = [torch.empty(w.shape, dtype=torch.bfloat16, device=device) for w in weights]  # the caller's stream's memory
+    side.wait_stream(main)
+    events = []
+    for w, o in zip(weights, outs):
+        o.record_stream(side)
+        _run(device, "mirai_mxfp4_dequantize", w.packed.data_ptr(), w.scale.data_ptr(), *w.shape, o.data_ptr(),
+             _MXFP4_DTYPES[torch.bfloat16], stream=side.cuda_stream)
+        events.append(side.record_event())
+    return outs, (lambda n: main.wait_event(events[n - 1]))
+
+
 def moe_forward_train(tokens, top_indices, top_weights, w1, w3, w2, *, num_experts: int, inter: int,
                       out_dtype: torch.dtype | None = None, lora: DownLoRA | None = None):
     """Forward that also returns the state the dX pass consumes."""
@@ -1208,7 +1259,10 @@ def moe_backward_dx(grad_out: torch.Tensor, state: ForwardState, w1, w3, w2, *, 
     grad_out [T, H] -> (dx [T, H], d_top_weights fp32 [T, k])."""
     plan = state.plan
     H = state.y_sorted.shape[1]
-    if state.staged is not None and all(a is b for a, b in zip(state.staged[0], (w1, w3, w2))):
+    mx = isinstance(w2, Mxfp4Tensor)
+    if mx:  # the stored values in bf16, w2 first, beside the combine backward and the down dX
+        dense, join = _read_back_beside((w2, w1, w3))
+    elif state.staged is not None and all(a is b for a, b in zip(state.staged[0], (w1, w3, w2))):
         w1, w3, w2 = state.staged[1]  # the forward's bf16 copies of these NF4 keys
         state.staged = None
     else:
@@ -1226,6 +1280,13 @@ def moe_backward_dx(grad_out: torch.Tensor, state: ForwardState, w1, w3, w2, *, 
                                     torch.empty((E, r, Ia), dtype=torch.float32, device=gy.device), (r * Ia, Ia, 1))
             lora.grad_b = lora_grad(gy, state.rank_a, plan.offsets, r,
                                     torch.empty((E, Hb, r), dtype=torch.float32, device=gy.device), (Hb * r, 1, r))
+    if mx:
+        join(1)
+        dgu = _down_dx_mxfp4(gy, plan.offsets, w2, state.gate_up, inter=inter, out=None, lora=lora, rank_a=glow, sources=1,
+                             dense=dense[0])
+        join(3)
+        dxs = gateup_dx(dgu, plan.offsets, dense[1], dense[2], hidden=H)
+        return combine(dxs, plan.inverse_order, None, out_dtype=out_dtype, top_k=plan.top_k), gw
     g_in, g_mid = _rotations(w1, w3, w2)
     if g_mid:  # rotated INT8: dh = rotate(grad_y (q s)), then the SwiGLU backward
         dh = down_dh(gy, plan.offsets, w2, inter=inter, lora=lora, rank_a=glow)
