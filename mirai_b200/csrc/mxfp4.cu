@@ -1457,6 +1457,9 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   int pairs = pairs_fit;
   if (limit > 0 && limit / 2 < pairs) pairs = limit / 2 > 0 ? limit / 2 : 1;
   const int64_t tiles = S / TILE_M + (segs < S ? segs : S);  // at most; about S / 256 when segments are long
+  if (tiles * p.n_tiles > INT32_MAX)
+    return set_error(MIRAI_ERR_UNSUPPORTED, "%s: %lld row tiles x %d column tiles are too many for one call", name,
+                     (long long)tiles, p.n_tiles);
   const int total_kb = (int)ceil_div(K, BKE) + p.has_ext;
   p.resident = total_kb <= A_BUFS;
   // Column tiles per unit: the run that makes the longest pair's time shortest, a tile counting its
