@@ -390,7 +390,6 @@ struct Params {
   int64_t S;
   int K, N;                // reduction length; output columns (I or H)
   int n_tiles;
-  int n_run;               // column tiles a unit walks over
   int w_blocks;            // row tiles of one expert's scales
   int has_ext;
   int a_bufs, b_stages;    // ring sizes
@@ -545,8 +544,11 @@ struct Ring {  // position in a ring of buffers
   }
 };
 
-// A unit of work: a row tile and a run of column tiles.  Unit u is run u / tiles of row
-// tile u % tiles, so that the pairs at work together share experts' B tiles in L2.
+// A unit of work: a row tile and a run of column tiles.  As many row tiles as fill every
+// pair equally often are walked whole; the rest are cut into runs, as long as they
+// keep the pairs that end last short, so that all pairs end together (whole row tiles
+// alone leave a third of the pairs idle for a quarter of the 32768-token layer).  Runs
+// are the outer index: the pairs at work together share experts' B tiles in L2.
 // One warp decodes units ahead of their use into a ring of shared memory: decoding in
 // every role cost 2 us at each change of unit.
 struct Unit {
@@ -555,9 +557,36 @@ struct Unit {
   int blk;       // first of the tile's two scale blocks
   int n0, n1;
 };
-__device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Params& p) {
-  const int tiles = tb.tile_prefix[p.segs];
-  const int run = u / tiles, mt = u - run * tiles;
+struct Schedule {
+  int whole;  // units of a whole row tile
+  int rest;   // row tiles cut into runs
+  int run;    // column tiles of a run
+  int units;
+};
+// By a whole warp: each lane weighs some lengths, a tile counting its B stream and a unit half a
+// tile more for its A.  Streamed A (not resident) makes every tile a unit.
+__device__ __forceinline__ Schedule make_schedule(int tiles, int pairs, const Params& p) {
+  Schedule s;
+  s.whole = p.resident ? tiles / pairs * pairs : 0;
+  s.rest = tiles - s.whole;
+  uint32_t best = 0xffffffffu;
+  for (int r = (threadIdx.x & 31) + 1; r <= (p.resident ? p.n_tiles : 1); r += 32) {
+    const int64_t rounds = ((int64_t)s.rest * ((p.n_tiles + r - 1) / r) + pairs - 1) / pairs;
+    const uint32_t cost = (uint32_t)min((int64_t)0x3fffff, rounds * (2 * r + 1));
+    best = min(best, cost << 10 | (uint32_t)min(r, 1023));  // the shortest run of the cheapest
+  }
+  s.run = (int)(__reduce_min_sync(0xffffffffu, best) & 1023u);
+  s.units = s.whole + s.rest * ((p.n_tiles + s.run - 1) / s.run);
+  return s;
+}
+__device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Schedule& s, const Params& p) {
+  int mt = u, n0 = 0, n1 = p.n_tiles;
+  if (u >= s.whole) {
+    const int run = (u - s.whole) / s.rest;
+    mt = s.whole + (u - s.whole) - run * s.rest;
+    n0 = run * s.run;
+    n1 = min(p.n_tiles, n0 + s.run);
+  }
   int lo = 0, hi = p.segs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -565,8 +594,7 @@ __device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Params
     else hi = mid;
   }
   const int m = mt - tb.tile_prefix[lo];
-  return Unit{tb.row_start[lo] + m * TILE_M, tb.row_start[lo + 1], lo % p.experts, tb.blk_prefix[lo] + 2 * m,
-              run * p.n_run, min(p.n_tiles, (run + 1) * p.n_run)};
+  return Unit{tb.row_start[lo] + m * TILE_M, tb.row_start[lo + 1], lo % p.experts, tb.blk_prefix[lo] + 2 * m, n0, n1};
 }
 // The next unit, false after the last one (or a wait that gave up).  `lanes` of the
 // warp call it together; the first of them frees the slot.
@@ -653,16 +681,16 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp < SF_FIRST) {
     regs_dec<REG_LOW>();
-    if (warp == 3 && lane == 0) {
+    if (warp == 3) {
       // ======================= unit scheduler =======================
       const int pairs = (int)(gridDim.x >> 1);
-      const int num_units = tb.tile_prefix[p.segs] * ((p.n_tiles + p.n_run - 1) / p.n_run);
+      const Schedule sched = make_schedule(tb.tile_prefix[p.segs], pairs, p);
       Ring r;
-      for (int u = (int)(blockIdx.x >> 1);; u += pairs) {
-        const bool more = u < num_units;
+      for (int u = (int)(blockIdx.x >> 1); lane == 0; u += pairs) {
+        const bool more = u < sched.units;
         Unit un = {};
         if (more) {
-          un = decode_unit(tb, u, p);
+          un = decode_unit(tb, u, sched, p);
           // The pairs change row tiles at about the same time: bring the rows into L2 ahead of that
           // burst (19 MB at 148 SMs).  (Boxes that reach past the last row are left out: prefetching
           // them took 17 us of a 16-row call.)
@@ -1457,29 +1485,17 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   int pairs = pairs_fit;
   if (limit > 0 && limit / 2 < pairs) pairs = limit / 2 > 0 ? limit / 2 : 1;
   const int64_t tiles = S / TILE_M + (segs < S ? segs : S);  // at most; about S / 256 when segments are long
-  if (tiles * p.n_tiles > INT32_MAX)
+  if (tiles * p.n_tiles > INT32_MAX || p.n_tiles > 1023)
     return set_error(MIRAI_ERR_UNSUPPORTED, "%s: %lld row tiles x %d column tiles are too many for one call", name,
                      (long long)tiles, p.n_tiles);
   const int total_kb = (int)ceil_div(K, BKE) + p.has_ext;
   p.resident = total_kb <= A_BUFS;
-  // Column tiles per unit: the run that makes the longest pair's time shortest, a tile counting its
-  // B stream and a unit half a tile more for its A.  (The row tiles are known on the device only: a
-  // segment's last one is half full on average.)
-  const int64_t likely = S / TILE_M + (segs < S ? (segs + 1) / 2 : S);
-  p.n_run = 1;
-  if (p.resident) {
-    double best = 0;
-    for (int r = 1; r <= p.n_tiles; ++r) {
-      const double cost = (double)ceil_div(likely * ceil_div(p.n_tiles, r), pairs) * (r + 0.5);
-      if (r == 1 || cost < best) best = cost, p.n_run = r;
-    }
-  }
   // Rings: A whole where it fits, the rest for B.  (More A buffers, to start the next unit's rows
   // early, measured slower than the B stages they take: 125 against 113 us for the layer's down.)
   p.a_bufs = p.resident ? (total_kb < 4 ? 4 : total_kb) : 5;
   p.b_stages = B_STAGES;
   while (smem_bytes(p.a_bufs, p.b_stages, p.segs) > kSmemLimit) --p.b_stages;
-  int64_t units = tiles * ceil_div(p.n_tiles, p.n_run);
+  int64_t units = tiles * p.n_tiles;
   if (units > pairs) units = pairs;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(THREADS, 1, 1);
