@@ -3,7 +3,7 @@
  *
  * This library replaces the routed expert FFN of seruva19/mirai: fp32 router
  * top-k, expert-contiguous token permute, SwiGLU gate/up and down grouped GEMMs
- * over frozen bf16 / NF4 / INT8 expert weights, the weighted un-permute
+ * over frozen bf16 / NF4 / INT8 / MXFP4 expert weights, the weighted un-permute
  * (combine), and the input-gradient (dX) path through the frozen experts.
  *
  * Conventions shared by every entry point:
