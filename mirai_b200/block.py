@@ -23,7 +23,9 @@ Two ways to use this module:
 
 Expert selection is the sm_100a router kernel; the routing weights that carry
 gradients back into the router are recomputed in torch from the selected
-indices (an elementwise [T, k] gather), so the router stays trainable.
+indices (an elementwise [T, k] gather), so the router stays trainable.  With
+``num_groups`` > 1 a token's experts come from its best groups, and selection
+and gradient are one kernel each (``ops.route_groups``).
 """
 
 from __future__ import annotations
@@ -33,6 +35,7 @@ from typing import Any, Callable, Mapping
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .backend import B200MoEKernelBackend
@@ -172,6 +175,7 @@ class _GroupRouteFunction(torch.autograd.Function):
         return idx, w
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, _, grad_w):
         logits, idx = ctx.saved_tensors
         grad = ops.route_groups_backward(grad_w.float(), logits, idx, **ctx.weighting)

@@ -540,10 +540,12 @@ MXFP4_FEW_ROWS_PER_SEGMENT = 16
 _FEW_MAX_ROWS, _FEW_MAX_WIDTH = 1024, 4096
 
 
+def _few_limit(segments: int) -> int:
+    return min(_FEW_MAX_ROWS, max(MXFP4_FEW_ROWS, MXFP4_FEW_ROWS_PER_SEGMENT * segments))
+
+
 def _few_rows(x, width: int, segments: int) -> bool:
-    if not isinstance(x, torch.Tensor) or width > _FEW_MAX_WIDTH:
-        return False
-    return x.shape[0] <= min(_FEW_MAX_ROWS, max(MXFP4_FEW_ROWS, MXFP4_FEW_ROWS_PER_SEGMENT * segments))
+    return isinstance(x, torch.Tensor) and width <= _FEW_MAX_WIDTH and x.shape[0] <= _few_limit(segments)
 
 
 def _few_input(x: torch.Tensor, width: int, name: str) -> torch.Tensor:
@@ -1106,10 +1108,15 @@ def moe_forward(tokens: torch.Tensor, top_indices: torch.Tensor, top_weights: to
 
 def _mxfp4_experts(tokens, plan: DispatchPlan, w1, w3, w2, *, inter: int, lora: DownLoRA | None, train: bool):
     """(y, gate_up, h, rank_a) of the routed rows in MXFP4: quantised in the
-    permute's pass, h in the gate/up epilogue.  gate_up when ``train``; h and
-    rank_a with a LoRA adapter, whose projection reads h in bf16."""
+    permute's pass, h in the gate/up epilogue (a generation step's few rows inside
+    the products).  gate_up when ``train``; h and rank_a with a LoRA adapter,
+    whose projection reads h in bf16."""
     if not all(isinstance(w, Mxfp4Tensor) for w in (w1, w3, w2)):
         raise TypeError("MXFP4 experts hold all three keys in MXFP4")
+    if lora is None and plan.total_slots <= _few_limit(plan.offsets.numel()) and max(tokens.shape[1], inter) <= _FEW_MAX_WIDTH:
+        rows = permute_rows(tokens, plan.sorted_token_indices)
+        h, gu, _ = _gateup_mxfp4(rows, plan.offsets, w1, w3, inter=inter, save_gate_up=train, want_h=True, want_rows=False)
+        return down(h, plan.offsets, w2, hidden=tokens.shape[1]), gu, None, None
     rows = mxfp4_quantize_rows(tokens, plan.offsets, row_index=plan.sorted_token_indices)
     h, gu, hq = _gateup_mxfp4(rows, plan.offsets, w1, w3, inter=inter, save_gate_up=train, want_h=lora is not None,
                               want_rows=True)

@@ -552,6 +552,29 @@ def test_experts_forward_and_backward(T, E, k, H, I):
     assert rel(out, ro) < 0.02 and rel(x.grad, rx) < 0.01 and rel(score.grad, rs) < 0.02
 
 
+def test_a_layer_runs_either_kernel_alike(monkeypatch):
+    """A generation step's rows through the few-row products and through the general ones: the same accumulations."""
+    dev = _dev()
+    from mirai_b200 import ops
+    E, T, k, H, I = 6, 9, 2, 320, 160
+    g = torch.Generator().manual_seed(2)
+    w1, w3 = ops.mxfp4_quantize(weight(E, I, H, dev, 1)), ops.mxfp4_quantize(weight(E, I, H, dev, 2))
+    w2 = ops.mxfp4_quantize(weight(E, H, I, dev, 3))
+    x = rows(T, H, dev)
+    idx = torch.rand(T, E, generator=g).topk(k, dim=1).indices.to(dev)
+    score = torch.rand(T, k, generator=g).to(dev)
+    few = ops.moe_forward(x, idx, score, w1, w3, w2, num_experts=E, inter=I)
+    before = ops.launch_count()
+    ops.moe_forward(x, idx, score, w1, w3, w2, num_experts=E, inter=I)
+    assert ops.launch_count() - before == 4 + 4  # the plan, then permute, two products, combine
+    monkeypatch.setattr(ops, "MXFP4_FEW_ROWS", -1)
+    monkeypatch.setattr(ops, "MXFP4_FEW_ROWS_PER_SEGMENT", 0)
+    general = ops.moe_forward(x, idx, score, w1, w3, w2, num_experts=E, inter=I)
+    ops.check_device()
+    # both add the same exact products step by step in fp32: at most a rounding of y and of the sum apart
+    assert ((few.float() - general.float()).abs() <= 2.0 ** -7 * general.float().abs() + 2.0 ** -8 * general.float().abs().mean()).all()
+
+
 def test_layer_gradient_against_differences():
     """The gradient of the smooth part: rows the quantiser keeps as they are (values on the grid), w2 = an adapter-free
     down of one expert.  Differences of the 64-bit layer with the quantisers left out agree with the kernels'."""

@@ -167,7 +167,7 @@ def grad64(gw, logits, idx, score_func, norm, scale):
     return torch.autograd.grad(w, lg, gw.double())[0], s.detach()
 
 
-@pytest.mark.parametrize("E,k", [(8, 2), (60, 3), (128, 8), (256, 8), (300, 1), (1024, 16)])
+@pytest.mark.parametrize("E,k", [(8, 2), (60, 3), (91, 9), (128, 8), (135, 7), (256, 8), (300, 1), (1023, 4), (1024, 16)])
 @pytest.mark.parametrize("score_func,norm", GRADS)
 def test_route_groups_gradient(E, k, score_func, norm):
     dev = _dev()
@@ -234,6 +234,43 @@ def test_gradient_of_masked_rows_and_repeated_ids():
     got = ops.route_groups_backward(gw.to(dev), lg.to(dev), idx.to(dev))
     assert ops.device_status() == (5, 750)
     assert torch.isfinite(got).all()
+
+
+def test_unaligned_rows_other_streams_and_graphs():
+    """Logits and bias that start off 16 bytes, two streams at once, and a captured route replayed on new logits."""
+    dev = _dev()
+    from mirai_b200 import ops
+    T, E, k = 300, 64, 6
+    g = torch.Generator().manual_seed(9)
+    xs = [torch.randn(T, E, generator=g).to(dev) for _ in range(4)]
+    bias = torch.randn(E, generator=g).to(dev) * 0.1
+    kw = {"num_groups": 8, "top_groups": 3, "choice_bias": bias}
+    want = [ops.route_groups(x, k, **kw) for x in xs]
+    grads = [ops.route_groups_backward(w, x, i) for x, (i, w) in zip(xs, want)]
+    store, bstore = torch.zeros(T * E + 1, device=dev), torch.zeros(E + 1, device=dev)
+    store[1:], bstore[1:] = xs[0].flatten(), bias
+    off = store[1:].view(T, E)
+    idx, w = ops.route_groups(off, k, **dict(kw, choice_bias=bstore[1:]))
+    assert torch.equal(idx, want[0][0]) and torch.equal(w, want[0][1])
+    assert torch.equal(ops.route_groups_backward(w, off, idx), grads[0])
+    turned = xs[1].t().contiguous().t()
+    assert torch.equal(ops.route_groups(turned, k, **kw)[0], want[1][0])
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i, x in enumerate(xs):
+        streams[i % 2].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(ops.route_groups(x, k, **kw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) for a, b in zip(got, want))
+    static, graph = xs[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        idx, w = ops.route_groups(static, k, **kw)
+        gl = ops.route_groups_backward(w, static, idx)
+    for x, (i, v), d in zip(xs, want, grads):
+        static.copy_(x)
+        graph.replay()
+        assert torch.equal(idx, i) and torch.equal(w, v) and torch.equal(gl, d)
+    ops.check_device()
 
 
 def test_block_routes_by_groups_with_its_gradient():
