@@ -183,6 +183,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
                                                        uint8_t* __restrict__ scale) {
   const int strip = blockIdx.x % (kBlockRows / kStrip);
   const int blk = blockIdx.x / (kBlockRows / kStrip);
+  // a product launched behind this kernel may set itself up while the last blocks run (it waits for
+  // their results with griddepcontrol.wait)
+  if (ROWS) asm volatile("griddepcontrol.launch_dependents;");
   RowBlock b;
   if constexpr (ROWS) {
     b = find_block(offsets, nseg, S, blk);
@@ -632,7 +635,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
 
-  build_segments(tb, p.offsets, p.segs, p.S, 710 + MODE);
   if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < A_BUFS; ++i) {
@@ -668,6 +670,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       prefetch_tmap(&tmap_sb1);
     }
   }
+  // Nothing above touches global memory: the kernel may be launched before the one in front of it
+  // in the stream has ended.  Every thread waits for that one here.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  build_segments(tb, p.offsets, p.segs, p.S, 710 + MODE);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -1502,13 +1508,15 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   cfg.gridDim = dim3((unsigned)(2 * units), 1, 1);
   cfg.dynamicSmemBytes = smem_bytes(p.a_bufs, p.b_stages, p.segs);
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, product_kernel<MODE>, ta, tsa, tb0, tb1, tsb0, tsb1, txa, txb, to0, to1,
                                            to2, p);
   if (e != cudaSuccess) return set_error(MIRAI_ERR_CUDA, "%s: launch failed: %s", name, cudaGetErrorString(e));
