@@ -539,6 +539,13 @@ __device__ __forceinline__ void build_segments(const Table& tb, const int32_t* o
   }
 }
 
+// mbar_wait by a whole warp, with one answer: its lanes go on, or give up, together, so that the
+// warp-wide instructions behind it (tcgen05.ld / .st, shuffles) and a slot that lane 0 frees
+// for all of them never meet a part of the warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, where));
+}
+
 struct Ring {  // position in a ring of buffers
   int i = 0;
   uint32_t phase = 0;
@@ -599,19 +606,20 @@ __device__ __forceinline__ Unit decode_unit(const Table& tb, int u, const Schedu
   const int m = mt - tb.tile_prefix[lo];
   return Unit{tb.row_start[lo] + m * TILE_M, tb.row_start[lo + 1], lo % p.experts, tb.blk_prefix[lo] + 2 * m, n0, n1};
 }
-// The next unit, false after the last one (or a wait that gave up).  `lanes` of the
-// warp call it together; the first of them frees the slot.
-__device__ __forceinline__ bool next_unit(Smem& sm, Ring& r, Unit& u, int site) {
-  if (!mbar_wait(&sm.u_full[r.i], r.phase, site)) {
+// The next unit, false after the last one (or a wait that gave up).  WARP: the whole warp
+// calls it; otherwise one lane does.  The slot is freed once every caller has read it.
+template <bool WARP> __device__ __forceinline__ bool next_unit(Smem& sm, Ring& r, Unit& u, int site) {
+  if (!(WARP ? mbar_wait_warp(&sm.u_full[r.i], r.phase, site) : mbar_wait(&sm.u_full[r.i], r.phase, site))) {
     *(volatile int*)&sm.abort_flag = 1;
     return false;
   }
   const int4 a = sm.units[r.i][0], b = sm.units[r.i][1];
   u = Unit{a.x, a.y, a.z, a.w, b.x, b.y};
-  __syncwarp(__activemask());
-  if ((threadIdx.x & 31) == 0) mbar_arrive(&sm.u_empty[r.i]);
+  if (WARP) __syncwarp();
+  if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&sm.u_empty[r.i]);
   r.next(U_RING);
-  return b.z != 0 && !*(volatile int*)&sm.abort_flag;
+  const bool more = b.z != 0 && !*(volatile int*)&sm.abort_flag;
+  return WARP ? __all_sync(0xffffffffu, more) : more;
 }
 
 template <int MODE>
@@ -718,7 +726,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t a_full0 = mapa_shared(smem_u32(&sm.a_full[0]), 0), b_full0 = mapa_shared(smem_u32(&sm.b_full[0]), 0);
       Ring ra, rb, ru;
       Unit un;
-      while (next_unit(sm, ru, un, 80)) {
+      while (next_unit<false>(sm, ru, un, 80)) {
         const int e = un.expert, row = un.row + (int)rank * BM;
         const CUtensorMap* mb = MODE == GATEUP && rank ? &tmap_b1 : &tmap_b0;
         for (int n = un.n0; n < un.n1 && !*abort_flag; ++n) {
@@ -758,7 +766,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ======================= TMA producer of the scales =======================
       Ring rb, ru;
       Unit un;
-      while (next_unit(sm, ru, un, 81)) {
+      while (next_unit<false>(sm, ru, un, 81)) {
         const int e = un.expert, ablk = un.blk + (int)rank;
         for (int n = un.n0; n < un.n1 && !*abort_flag; ++n) {
           // row tiles of both column halves
@@ -796,18 +804,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint32_t acc = 0;  // all 512 columns are this CTA's: they start at 0 (checked above)
       uint32_t tiles = 0;
       bool ok = true;
-      while (ok && next_unit(sm, ru, un, 82)) {
+      while (ok && next_unit<true>(sm, ru, un, 82)) {
         const Ring ra0 = ra;
         for (int n = un.n0; n < un.n1 && ok; ++n, ++tiles) {
           if (p.resident) ra = ra0;
           const bool first = n == un.n0 || !p.resident, last = n + 1 == un.n1 || !p.resident;
           // (the first k-block's operands are waited for before the accumulator: they come first)
-          if ((first && !mbar_wait(&sm.a_full[ra.i], ra.phase, 75)) || !mbar_wait(&sm.b_full[rb.i], rb.phase, 76) ||
-              (tiles > 0 && !mbar_wait(&sm.tempty, (tiles - 1) & 1, 74)))
+          if ((first && !mbar_wait_warp(&sm.a_full[ra.i], ra.phase, 75)) ||
+              !mbar_wait_warp(&sm.b_full[rb.i], rb.phase, 76) ||
+              (tiles > 0 && !mbar_wait_warp(&sm.tempty, (tiles - 1) & 1, 74)))
             ok = false;
           for (int kb = 0; kb < total_kb && ok; ++kb) {
-            if (kb > 0 && ((first && !mbar_wait(&sm.a_full[ra.i], ra.phase, 75)) ||
-                           !mbar_wait(&sm.b_full[rb.i], rb.phase, 76))) {
+            if (kb > 0 && ((first && !mbar_wait_warp(&sm.a_full[ra.i], ra.phase, 75)) ||
+                           !mbar_wait_warp(&sm.b_full[rb.i], rb.phase, 76))) {
               ok = false;
               break;
             }
@@ -852,11 +861,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t b_full0 = mapa_shared(smem_u32(&sm.b_full[0]), 0);
     Ring rb, ru;
     Unit un;
-    while (next_unit(sm, ru, un, 83)) {
+    while (next_unit<true>(sm, ru, un, 83)) {
       const int blocks = (un.n1 - un.n0) * total_kb;
       int kb = 0;
       for (int i = 0; i < blocks; ++i) {
-        if (!mbar_wait(&sm.sf_full[rb.i], rb.phase, 77)) {
+        if (!mbar_wait_warp(&sm.sf_full[rb.i], rb.phase, 77)) {
           *abort_flag = 1;
           break;
         }
@@ -891,7 +900,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t tiles = 0;
     Ring ru;
     Unit un;
-    while (next_unit(sm, ru, un, 84)) {
+    while (next_unit<true>(sm, ru, un, 84)) {
       const int64_t row = (int64_t)un.row + (int)rank * BM + q * 32 + lane;
       const bool valid = row < un.end;
       const bool boxed = __all_sync(0xffffffffu, valid);  // all 32 rows are the segment's
@@ -920,7 +929,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       bool ok = true;
       for (int n = un.n0; n < un.n1 && ok; ++n, ++tiles) {
-        if (!mbar_wait(&sm.tfull, tiles & 1, 78)) {
+        if (!mbar_wait_warp(&sm.tfull, tiles & 1, 78)) {
           *abort_flag = 1;
           ok = false;
           break;
@@ -1192,10 +1201,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     Ring r;
     uint32_t done = 0;
     bool ok = true;
-    for (int t = (int)blockIdx.x; t < tiles && ok && !*abort_flag; t += gridDim.x, ++done) {
-      if (!mbar_wait(&sm.rows_ready, done & 1, 61) || (done > 0 && !mbar_wait(&sm.tempty, (done - 1) & 1, 62))) ok = false;
+    for (int t = (int)blockIdx.x; t < tiles && ok && !__any_sync(0xffffffffu, *abort_flag); t += gridDim.x, ++done) {
+      if (!mbar_wait_warp(&sm.rows_ready, done & 1, 61) ||
+          (done > 0 && !mbar_wait_warp(&sm.tempty, (done - 1) & 1, 62)))
+        ok = false;
       for (int kb = 0; kb < num_kb && ok; ++kb) {
-        if (!mbar_wait(&sm.full[r.i], r.phase, 63)) {
+        if (!mbar_wait_warp(&sm.full[r.i], r.phase, 63)) {
           ok = false;
           break;
         }
@@ -1224,7 +1235,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     if (!ok && lane == 0) *abort_flag = 1;
     // the last commits have arrived before the CTA frees its barriers and TMEM
     for (int i = 0; i < p.stages; ++i) {
-      if (!mbar_wait(&sm.empty[r.i], r.phase ^ 1, 64)) break;
+      if (!mbar_wait_warp(&sm.empty[r.i], r.phase ^ 1, 64)) break;
       r.next(p.stages);
     }
   } else if (warp >= 4) {
@@ -1232,10 +1243,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     const int q = warp & 3;
     Ring r;
     uint32_t done = 0;
-    for (int t = (int)blockIdx.x; t < tiles && !*abort_flag; t += gridDim.x, ++done) {
+    for (int t = (int)blockIdx.x; t < tiles && !__any_sync(0xffffffffu, *abort_flag); t += gridDim.x, ++done) {
       const Tile tl = decode(t);
       // the previous tile's MMAs have read the rows
-      if (done > 0 && !mbar_wait(&sm.tfull, (done - 1) & 1, 65)) {
+      if (done > 0 && !mbar_wait_warp(&sm.tfull, (done - 1) & 1, 65)) {
         *abort_flag = 1;
         break;
       }
@@ -1283,14 +1294,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       if (lane == 0) mbar_arrive(&sm.rows_ready);
       if (warp >= 8) continue;
       // every quantising warp's scale words are read here
-      if (!mbar_wait(&sm.rows_ready, done & 1, 68)) {
+      if (!mbar_wait_warp(&sm.rows_ready, done & 1, 68)) {
         *abort_flag = 1;
         break;
       }
       const uint32_t quarter = (uint32_t)(q * 32) << 16;
       bool ok = true;
       for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&sm.sf_full[r.i], r.phase, 66)) {
+        if (!mbar_wait_warp(&sm.sf_full[r.i], r.phase, 66)) {
           *abort_flag = 1;
           ok = false;
           break;
@@ -1308,7 +1319,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         r.next(p.stages);
       }
       if (!ok) break;
-      if (!mbar_wait(&sm.tfull, done & 1, 67)) {
+      if (!mbar_wait_warp(&sm.tfull, done & 1, 67)) {
         *abort_flag = 1;
         break;
       }
