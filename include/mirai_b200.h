@@ -584,7 +584,8 @@ int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_
 
 /* The expert products on MXFP4 operands (tcgen05 block-scaled MMAs, fp32 accumulation):
  * segment s * num_experts + e holds source s's rows of expert e, offsets ends all
- * num_sources * num_experts (<= 1024) of them.  hidden and inter are multiples of 32.
+ * num_sources * num_experts (<= 1024) of them.  hidden and inter are multiples of 32; gate/up
+ * takes inter up to 130944, down hidden up to 261888.
  *
  * gate/up: h = silu(g) * u, g = x W1^T, u = x W3^T, rounded once to bf16 from fp32.
  * h [S, I] bf16 and/or its quantised form (h_packed [S, I/2], h_scale: the segment-tiled

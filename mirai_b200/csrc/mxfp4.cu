@@ -1464,6 +1464,10 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   p.K = K;
   p.N = N;
   p.n_tiles = (int)ceil_div(N, MODE == GATEUP ? BM : TN);
+  const int64_t tiles = S / TILE_M + (segs < S ? segs : S);  // at most; about S / 256 when segments are long
+  if (tiles * p.n_tiles > INT32_MAX || p.n_tiles > 1023)
+    return set_error(MIRAI_ERR_UNSUPPORTED, "%s: %lld row tiles x %d column tiles are too many for one call", name,
+                     (long long)tiles, p.n_tiles);
   p.w_blocks = (int)ceil_div(N, kBlockRows);
   p.has_ext = rank_a != nullptr;
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -1501,10 +1505,6 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   const int limit = gemm_sm_limit();
   int pairs = pairs_fit;
   if (limit > 0 && limit / 2 < pairs) pairs = limit / 2 > 0 ? limit / 2 : 1;
-  const int64_t tiles = S / TILE_M + (segs < S ? segs : S);  // at most; about S / 256 when segments are long
-  if (tiles * p.n_tiles > INT32_MAX || p.n_tiles > 1023)
-    return set_error(MIRAI_ERR_UNSUPPORTED, "%s: %lld row tiles x %d column tiles are too many for one call", name,
-                     (long long)tiles, p.n_tiles);
   const int total_kb = (int)ceil_div(K, BKE) + p.has_ext;
   p.resident = total_kb <= A_BUFS;
   // Rings: A whole where it fits, the rest for B.  (More A buffers, to start the next unit's rows

@@ -114,6 +114,17 @@ def test_product_refusals(lib):
     refused(lib, 1, b"rank-block", x, ALIGNED, ALIGNED, 1, 4, 16, 64, 64, ALIGNED, ALIGNED, ALIGNED, None, ALIGNED, None)
 
 
+def test_a_product_too_wide_for_its_tiles_is_refused(lib):
+    """1023 column tiles at most: of 128 channels in gate/up, of 256 outputs in down."""
+    w = _lib.Mxfp4Weight(ALIGNED, ALIGNED)
+    refused(lib, 2, b"column tiles", "mirai_moe_gateup_swiglu_mxfp4", ALIGNED, ALIGNED, ALIGNED, 1, 4, 16, 64,
+            1023 * 128 + 32, w, w, ALIGNED, None, None, None, None)
+    refused(lib, 2, b"column tiles", "mirai_moe_down_mxfp4", ALIGNED, ALIGNED, ALIGNED, 1, 4, 16, 64, 1023 * 256 + 32, w,
+            None, None, ALIGNED, None)
+    refused(lib, 2, b"row tiles", "mirai_moe_down_mxfp4", ALIGNED, ALIGNED, ALIGNED, 1, 1, (1 << 31) - 257, 64,
+            1023 * 256, w, None, None, ALIGNED, None)  # 2^23 x 1023 tiles
+
+
 def test_route_groups_refusals(lib):
     r = "mirai_route_groups"
     ok = [ALIGNED, 1, 8, 64, 4, 8, 3, 1, 1, None, 2, 1.0, ALIGNED, ALIGNED, None]
