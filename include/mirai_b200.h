@@ -590,7 +590,7 @@ int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_
  * gate/up: h = silu(g) * u, g = x W1^T, u = x W3^T, rounded once to bf16 from fp32.
  * h [S, I] bf16 and/or its quantised form (h_packed [S, I/2], h_scale: the segment-tiled
  * scales of width I), of the bf16-rounded h; gate_up (may be NULL) [S, 2I] bf16 is saved for
- * the backward.  down: y [S, H] = h W2^T; rank_a [S, 64] / rank_b [E*H, 64] bf16 (both or
+ * the backward (in bf16: see mirai_moe_gateup_swiglu_mxfp4_save).  down: y [S, H] = h W2^T; rank_a [S, 64] / rank_b [E*H, 64] bf16 (both or
  * neither) add a LoRA adapter's rank block, as in mirai_moe_down_lora_bf16.  The backward of
  * both multiplies the read-back weights (mirai_moe_down_dx_f32_bf16, mirai_moe_gateup_dx_bf16). */
 int mirai_moe_gateup_swiglu_mxfp4(const uint8_t* x_packed, const uint8_t* x_scale, const int32_t* offsets,
@@ -608,6 +608,41 @@ int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const 
 int mirai_moe_down_dx_f32_bf16(const void* grad_y, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
                                int64_t num_rows, int32_t hidden, int32_t inter, const void* w2, const void* gate_up,
                                const void* rank_a, const void* rank_b, void* grad_gate_up, mirai_stream_t stream);
+
+/* gate/up with the saved gate_up in a type of the caller's: gate_up_dtype MIRAI_DTYPE_BF16 (as
+ * mirai_moe_gateup_swiglu_mxfp4) or _F32, the accumulator itself (mirai_moe_gateup_swiglu_mxfp4_few_save: the
+ * few-row form below). */
+int mirai_moe_gateup_swiglu_mxfp4_save(const uint8_t* x_packed, const uint8_t* x_scale, const int32_t* offsets,
+                                       int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
+                                       int32_t inter, const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3,
+                                       void* h, void* gate_up, int32_t gate_up_dtype, uint8_t* h_packed,
+                                       uint8_t* h_scale, mirai_stream_t stream);
+int mirai_moe_gateup_swiglu_mxfp4_few_save(const void* x, const int32_t* offsets, int32_t num_sources,
+                                           int32_t num_experts, int64_t num_rows, int32_t hidden, int32_t inter,
+                                           const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3, void* h,
+                                           void* gate_up, int32_t gate_up_dtype, mirai_stream_t stream);
+
+/* The backward of an MXFP4 layer with its intermediates in fp32 (at most 1024 segments):
+ *   combine_backward_rows  grad_rows [S, H] bf16 = grad_out's row of each route, as it is; row_weights
+ *                          [S] fp32 = the routing weight of each row; grad_weights [T, k] as
+ *                          mirai_moe_combine_backward.
+ *   down_dx_rows_f32       mirai_moe_down_dx_f32_bf16 of grad_rows with gate_up in fp32 and the product
+ *                          (rank block included) multiplied by row_weights (may be NULL: 1) in fp32.
+ *   gateup_dx_f32          mirai_moe_gateup_dx_bf16 (any number of sources) with dx in fp32.
+ *   combine_f32            mirai_moe_combine of fp32 rows (out_dtype MIRAI_DTYPE_BF16 or _F32). */
+int mirai_moe_combine_backward_rows(const void* grad_out, const void* y_sorted, const int64_t* inverse_order,
+                                    const float* top_weights, int64_t num_tokens, int32_t top_k, int32_t hidden,
+                                    void* grad_rows, float* row_weights, float* grad_weights, mirai_stream_t stream);
+int mirai_moe_down_dx_rows_f32(const void* grad_rows, const float* row_weights, const int32_t* offsets,
+                               int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
+                               int32_t inter, const void* w2, const float* gate_up, const void* rank_a,
+                               const void* rank_b, void* grad_gate_up, mirai_stream_t stream);
+int mirai_moe_gateup_dx_f32(const void* grad_gate_up, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                            int64_t num_rows, int32_t inter, int32_t hidden, const void* w1, const void* w3,
+                            float* dx_sorted, mirai_stream_t stream);
+int mirai_moe_combine_f32(const float* y_sorted, const int64_t* inverse_order, const float* top_weights,
+                          int64_t num_tokens, int32_t top_k, int32_t hidden, void* out, int32_t out_dtype,
+                          mirai_stream_t stream);
 
 /* The same products for at most MIRAI_MXFP4_FEW_ROWS rows given in bf16 (32-byte aligned), of
  * at most 4096 elements: quantised in the kernel, which reads the weights of the experts that

@@ -185,6 +185,18 @@ SIGNATURES = {
     "mirai_moe_gateup_swiglu_mxfp4_few": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
                                                          ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight),
                                                          c_vp, c_vp, c_vp]),
+    "mirai_moe_gateup_swiglu_mxfp4_save": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
+                                                          ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight),
+                                                          c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
+    "mirai_moe_gateup_swiglu_mxfp4_few_save": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,
+                                                              ctypes.POINTER(Mxfp4Weight), ctypes.POINTER(Mxfp4Weight),
+                                                              c_vp, c_vp, c_i32, c_vp]),
+    "mirai_moe_combine_backward_rows": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp,
+                                                       c_vp]),
+    "mirai_moe_combine_f32": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_vp]),
+    "mirai_moe_down_dx_rows_f32": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp,
+                                                  c_vp, c_vp, c_vp, c_vp]),
+    "mirai_moe_gateup_dx_f32": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp]),
     "mirai_moe_down_dx_f32_bf16": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp,
                                                   c_vp, c_vp]),
     "mirai_moe_down_mxfp4_few": (ctypes.c_int, [c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32,

@@ -159,13 +159,14 @@ struct Params {
   int out_rows;            // K-major modes: rows of one expert's B matrix per key
   __nv_bfloat16* out;      // h [S,I] | y [S,H] | dgu [S,2I] | dx [S,H]
   int64_t ldo;             // elements
-  __nv_bfloat16* gate_up;  // GATEUP: optional saved [S,2I] output; DXDOWN: saved input
+  __nv_bfloat16* gate_up;  // GATEUP: optional saved [S,2I] output; DXDOWN: saved input (F32: fp32 values)
   QKey q[2];               // quantised keys (index 1 used by GATEUP / DXGATEUP)
   int nbs_shift;           // log2(nested_blocksize)
   int has_ext;             // 1: one extra bf16 k-block (the LoRA rank block) from tmap_xa / tmap_xb
   int nsrc;                // row sources: segment s*(E/nsrc) + w holds source s's rows for weight expert w
   int act;                 // Act of the gate/up epilogue (GATEUP) and of its backward (DXDOWN)
   int prev_end;            // 1: segment 0 starts at offsets[-1] (a later chunk of > kMaxExperts groups)
+  const float* row_scale;  // F32 DXDOWN: optional [S], dh is multiplied by it in fp32
 };
 
 // Control block in shared memory.  16-byte aligned size: the dequantiser
@@ -365,7 +366,12 @@ __device__ __forceinline__ int kmajor_row(const Params& p, int e, int n, int h) 
   return MODE == GATEUP ? e * p.out_rows + n * (TN / 2) : e * p.out_rows + n * TN + h * (TN / 2);
 }
 
-template <int MODE, int WF, bool PAIR, bool BMN>
+// F32 (the dX modes on bf16 weights): what lies between the GEMMs of the MXFP4 layer's backward and
+// need not be an MMA operand stays in fp32 -- DXDOWN reads the saved gate/up in fp32 and multiplies the
+// accumulator by the row's routing weight (its A rows are the output gradient as it came), DXGATEUP
+// writes dx [S, H] in fp32.  Each of the three in bf16 costs the layer's dx one more bf16 rounding
+// (0.0017 in the 2-norm; 0.0039 with the three, 0.0024 without).
+template <int MODE, int WF, bool PAIR, bool BMN, bool F32>
 __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b0,
                         const __grid_constant__ CUtensorMap tmap_b1, const __grid_constant__ CUtensorMap tmap_xa,
@@ -386,6 +392,7 @@ __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
   using MC = MCfg<MODE>;
   // B layouts other than the compressed-expert one run on CTA pairs only
   static_assert(PAIR || MN == MC::MN_NATIVE, "the transposed weight layout runs on CTA pairs");
+  static_assert(!F32 || (!QUANT && (MODE == DXDOWN || MODE == DXGATEUP)), "fp32 intermediates: bf16 dX GEMMs");
   // NF4 on CTA pairs: each tile's absmax codes reach one of two buffers a
   // tile ahead of use, so the dequantisers never stop to stage them.  K-major,
   // they are one contiguous run of B_ROWS x K/64 bytes, bulk-copied by the
@@ -692,8 +699,8 @@ __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
     const int part = (warp - C::EPI_FIRST) / 4;
     const uint32_t tempty_leader0 = leader_addr(&sm.tempty[0]), tempty_leader1 = leader_addr(&sm.tempty[1]);
     int stg = 0;  // the next staging box of this warp
-    // Write one 32 x 32 bf16 block (this lane's row: 16 packed words) through a
-    // staging box to `map` at (col, row0): the whole warp, rows row0..row0+31 all valid.
+    // Write one block of 32 rows x 32 bf16 columns, or 16 fp32 ones (this lane's row: 16 words), through
+    // a staging box to `map` at (col, row0): the whole warp, rows row0..row0+31 all valid.
     auto stage_store = [&](const CUtensorMap* map, int col, int64_t row0, const uint32_t (&w)[16]) {
       uint8_t* box = sStage + ((warp - C::EPI_FIRST) * STG_BUFS + stg) * STG_BOX;
       if (lane == 0) bulk_wait_group_read<STG_BUFS - 1>();  // the box's previous store has read it
@@ -731,9 +738,10 @@ __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
           const bool live = p.nsrc > 1 ? lr < blk_rows : (int64_t)m * TILE_M + r < seg_rows;
           if (!live || part != 0) continue;
           const int64_t grow = p.nsrc > 1 ? (int64_t)blk_row + lr : (int64_t)sm.row_start[j] + (int64_t)m * TILE_M + r;
-          const __nv_bfloat16* base = p.gate_up + grow * 2 * (int64_t)p.N + col0;
-          prefetch_l2_bulk(base, (uint32_t)cols * 2u);
-          prefetch_l2_bulk(base + p.N, (uint32_t)cols * 2u);
+          constexpr int GB = F32 ? 4 : 2;  // bytes of a saved value
+          const char* base = reinterpret_cast<const char*>(p.gate_up) + (grow * 2 * (int64_t)p.N + col0) * GB;
+          prefetch_l2_bulk(base, (uint32_t)(cols * GB));
+          prefetch_l2_bulk(base + (int64_t)p.N * GB, (uint32_t)(cols * GB));
         }
       }
       if (!mbar_wait(&sm.tfull[acc], acc_phase, 30)) {
@@ -801,6 +809,71 @@ __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
                 gd[v] = make_uint4(gp[4 * v], gp[4 * v + 1], gp[4 * v + 2], gp[4 * v + 3]);
                 ud[v] = make_uint4(up[4 * v], up[4 * v + 1], up[4 * v + 2], up[4 * v + 3]);
               }
+            }
+          }
+        }
+      } else if constexpr (MODE == DXDOWN && F32) {
+        // The same SwiGLU backward, all of it in fp32: dh = row weight * accumulator, one
+        // rounding of dgate and dup.  16 columns of the saved values are loaded ahead.
+        const int64_t ld2 = 2 * (int64_t)p.N;
+        const float rs = p.row_scale != nullptr && valid ? p.row_scale[grow] : 1.f;
+        constexpr int NCH = TN / 32;
+        const int c_first = part * (NCH / NSPLIT), c_end = (part + 1) * (NCH / NSPLIT);
+        float4 gnext[4], unext[4];
+        auto load_gu = [&](int h) {  // half chunk h: columns 16 h .. 16 h + 15 of the tile
+          const int col = n * TN + h * 16;
+          if (valid && col < p.N) {
+            const float* gs = reinterpret_cast<const float*>(p.gate_up) + grow * ld2 + col;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              gnext[v] = reinterpret_cast<const float4*>(gs)[v];
+              unext[v] = reinterpret_cast<const float4*>(gs + p.N)[v];
+            }
+          }
+        };
+        load_gu(2 * c_first);
+#pragma unroll 1
+        for (int c = c_first; c < c_end; ++c) {
+          const int col = n * TN + c * 32;
+          uint32_t v32[32], dg[16], du[16];
+          tmem_ld_32x32b_x32(tb + c * 32, v32);
+          tmem_ld_wait();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float gw[16], uw[16];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              gw[4 * v] = gnext[v].x, gw[4 * v + 1] = gnext[v].y, gw[4 * v + 2] = gnext[v].z, gw[4 * v + 3] = gnext[v].w;
+              uw[4 * v] = unext[v].x, uw[4 * v + 1] = unext[v].y, uw[4 * v + 2] = unext[v].z, uw[4 * v + 3] = unext[v].w;
+            }
+            if (h == 0 || c + 1 < c_end) load_gu(2 * c + h + 1);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float dgo[2], duo[2];
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const float dh = rs * __uint_as_float(v32[16 * h + 2 * j + z]);
+                const float gv = gw[2 * j + z], uv = uw[2 * j + z];
+                const float sg = __fdividef(1.f, 1.f + __expf(-gv));
+                duo[z] = dh * gv * sg;
+                dgo[z] = dh * uv * sg * (1.f + gv * (1.f - sg));
+              }
+              dg[8 * h + j] = pack_bf16x2(dgo[0], dgo[1]);
+              du[8 * h + j] = pack_bf16x2(duo[0], duo[1]);
+            }
+          }
+          if (valid && col < p.N) {
+            if (boxed) {
+              stage_store(&tmap_o0, col, row0, dg);  // the gate half of dgu
+              stage_store(&tmap_o1, col, row0, du);  // the up half
+              continue;
+            }
+            uint4* gd = reinterpret_cast<uint4*>(p.out + grow * ld2 + col);
+            uint4* ud = reinterpret_cast<uint4*>(p.out + grow * ld2 + p.N + col);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              gd[v] = make_uint4(dg[4 * v], dg[4 * v + 1], dg[4 * v + 2], dg[4 * v + 3]);
+              ud[v] = make_uint4(du[4 * v], du[4 * v + 1], du[4 * v + 2], du[4 * v + 3]);
             }
           }
         }
@@ -916,6 +989,24 @@ __global__ void __launch_bounds__(Cfg<WF, PAIR>::THREADS, 1)
           tmem_ld_32x32b_x32(tb + c * 32, v32);
           tmem_ld_wait();
           if (valid && col0 + c * 32 < p.N) {
+            if constexpr (F32) {  // two boxes of 16 fp32 columns
+              float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + grow * p.ldo + col0 + c * 32);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = v32[16 * h + j];
+                if (boxed) {
+                  stage_store(&tmap_o0, col0 + c * 32 + 16 * h, row0, w);
+                  continue;
+                }
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                  dst[4 * h + v] = make_float4(__uint_as_float(w[4 * v]), __uint_as_float(w[4 * v + 1]),
+                                               __uint_as_float(w[4 * v + 2]), __uint_as_float(w[4 * v + 3]));
+              }
+              continue;
+            }
             uint32_t yp[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) yp[j] = pack_bf16x2(__uint_as_float(v32[2 * j]), __uint_as_float(v32[2 * j + 1]));
@@ -1283,12 +1374,12 @@ static bool use_pairs() {
   return v == 1;
 }
 
-template <int MODE, int WF, bool PAIR, bool BMN>
+template <int MODE, int WF, bool PAIR, bool BMN, bool F32>
 int launch_impl(const CUtensorMap& ta, const CUtensorMap& tb0, const CUtensorMap& tb1, const CUtensorMap& txa,
                 const CUtensorMap& txb, const CUtensorMap* to, const Params& p,
                 cudaStream_t stream) {
   using C = Cfg<WF, PAIR>;
-  auto kern = grouped_gemm_kernel<MODE, WF, PAIR, BMN>;
+  auto kern = grouped_gemm_kernel<MODE, WF, PAIR, BMN, F32>;
   constexpr size_t smem = smem_bytes<WF, PAIR>();
   static_assert(smem <= 232448, "shared memory budget exceeded");
   static bool attr_set = false;
@@ -1353,20 +1444,20 @@ int launch_impl(const CUtensorMap& ta, const CUtensorMap& tb0, const CUtensorMap
 // BMN: B read MN-major.  The compressed-expert layout ([E, out, in]) has its
 // native B layout per mode (every format, single CTAs or pairs); the MAGI-2
 // layout ([E, in, out]) reads the other way round, for bf16 and NF4, on pairs.
-template <int MODE, int WF, bool BMN>
+template <int MODE, int WF, bool BMN, bool F32 = false>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb0, const CUtensorMap& tb1, const CUtensorMap& txa,
            const CUtensorMap& txb, const CUtensorMap* to, const Params& p,
            cudaStream_t stream) {
   if constexpr (BMN == MCfg<MODE>::MN_NATIVE) {
-    return use_pairs() ? launch_impl<MODE, WF, true, BMN>(ta, tb0, tb1, txa, txb, to, p, stream)
-                       : launch_impl<MODE, WF, false, BMN>(ta, tb0, tb1, txa, txb, to, p, stream);
+    return use_pairs() ? launch_impl<MODE, WF, true, BMN, F32>(ta, tb0, tb1, txa, txb, to, p, stream)
+                       : launch_impl<MODE, WF, false, BMN, F32>(ta, tb0, tb1, txa, txb, to, p, stream);
   } else if constexpr (WF == W_INT8) {
     return set_error(MIRAI_ERR_UNSUPPORTED, "INT8 experts are read in the [E, out, in] layout only");
   } else {
     if (!use_pairs())
       return set_error(MIRAI_ERR_UNSUPPORTED, "the [E, in, out] weight layout runs on CTA pairs "
                        "(MIRAI_B200_CTA_PAIR=0 is set)");
-    return launch_impl<MODE, WF, true, BMN>(ta, tb0, tb1, txa, txb, to, p, stream);
+    return launch_impl<MODE, WF, true, BMN, false>(ta, tb0, tb1, txa, txb, to, p, stream);
   }
 }
 
@@ -1492,7 +1583,8 @@ struct RankBlock {
 template <int MODE>
 int run_groups(const char* name, const void* a, const int32_t* offsets, int E, int64_t S, int K, int N, void* out,
                void* gate_up, const WeightArg& w0, const WeightArg& w1, int rows, int cols, mirai_stream_t stream,
-               const RankBlock* ext, int nsrc, bool dh_only, bool mn, int act, bool prev_end) {
+               const RankBlock* ext, int nsrc, bool dh_only, bool mn, int act, bool prev_end, bool f32 = false,
+               const float* row_scale = nullptr) {
   Params p;
   CUtensorMap ta, t0, t1, txa, txb;
   const int box_rows = kmajor_box_rows(w0.fmt);
@@ -1500,6 +1592,7 @@ int run_groups(const char* name, const void* a, const int32_t* offsets, int E, i
   p.nsrc = nsrc;
   p.act = act;
   p.prev_end = prev_end ? 1 : 0;
+  p.row_scale = row_scale;
   if (!rc && ext) {
     if (!ext->a || !ext->b) rc = set_error(MIRAI_ERR_INVALID_ARG, "%s: null rank-block operand", name);
     if (!rc)
@@ -1539,8 +1632,11 @@ int run_groups(const char* name, const void* a, const int32_t* offsets, int E, i
     const bool dgu = MODE == DXDOWN && p.gate_up != nullptr;  // [S, 2N]: gate half, then up half
     const uint64_t ld = dgu ? 2 * (uint64_t)N : (uint64_t)N;
     char* o = static_cast<char*>(out);
-    rc = make_tmap_2d(&to[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, o, (uint64_t)N, (uint64_t)S, ld * 2, 32, 32,
-                      CU_TENSOR_MAP_SWIZZLE_64B);
+    rc = f32 && MODE == DXGATEUP
+             ? make_tmap_2d(&to[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, o, (uint64_t)N, (uint64_t)S, ld * 4, 16, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B)
+             : make_tmap_2d(&to[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, o, (uint64_t)N, (uint64_t)S, ld * 2, 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B);
     if (!rc)
       rc = dgu ? make_tmap_2d(&to[1], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, o + (size_t)N * 2, (uint64_t)N,
                               (uint64_t)S, ld * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)
@@ -1557,6 +1653,9 @@ int run_groups(const char* name, const void* a, const int32_t* offsets, int E, i
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   constexpr bool NAT = MCfg<MODE>::MN_NATIVE;
+  if constexpr (MODE == DXDOWN || MODE == DXGATEUP) {
+    if (f32) return launch<MODE, W_BF16, NAT, true>(ta, t0, t1, txa, txb, to, p, st);  // (bf16 keys, native layout: see run_f32)
+  }
   switch (w0.fmt) {
     case W_BF16:
       return mn == NAT ? launch<MODE, W_BF16, NAT>(ta, t0, t1, txa, txb, to, p, st)
@@ -1629,6 +1728,20 @@ int run(const char* name, const void* a, const int32_t* offsets, int E, int64_t 
   }
   return run_groups<MODE>(name, a, offsets, E, S, K, N, out, gate_up, w0, w1, rows, cols, stream, ext, nsrc, dh_only,
                           mn, act, false);
+}
+
+// The dX modes with fp32 intermediates, on bf16 [E, out, in] weights; at most kMaxExperts segments.
+template <int MODE>
+static int run_f32(const char* name, const void* a, const int32_t* offsets, int nsrc, int E, int64_t S, int K, int N,
+                   void* out, void* gate_up, const void* w0, const void* w1, int rows, int cols, mirai_stream_t stream,
+                   const RankBlock* ext, const float* row_scale) {
+  if (nsrc <= 0 || E <= 0 || (int64_t)nsrc * E > kMaxExperts)
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: %d sources x %d experts outside 1..%d segments", name, nsrc, E,
+                     kMaxExperts);
+  if (S == 0) return MIRAI_OK;
+  const WeightArg k0{W_BF16, w0, nullptr, nullptr}, k1{W_BF16, w1, nullptr, nullptr};
+  return run_groups<MODE>(name, a, offsets, E, S, K, N, out, gate_up, k0, k1, rows, cols, stream, ext, nsrc, false,
+                          MCfg<MODE>::MN_NATIVE, ACT_SWIGLU, false, true, row_scale);
 }
 
 inline WeightArg wb(const void* w) { return WeightArg{W_BF16, w, nullptr, nullptr}; }
@@ -1823,6 +1936,22 @@ int mirai_moe_down_dx_f32_bf16(const void* grad_y, const int32_t* offsets, int32
   return run<DXDOWN>("down_dx_f32_bf16", grad_y, offsets, num_experts, num_rows, hidden, inter, grad_gate_up,
                      const_cast<void*>(gate_up), wb(w2), wb(w2), hidden, inter, stream, rank_a ? &rb : nullptr,
                      num_sources, false, -1, ACT_SWIGLU_F32);
+}
+int mirai_moe_down_dx_rows_f32(const void* grad_rows, const float* row_weights, const int32_t* offsets,
+                               int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
+                               int32_t inter, const void* w2, const float* gate_up, const void* rank_a,
+                               const void* rank_b, void* grad_gate_up, mirai_stream_t stream) {
+  if (!rank_a != !rank_b) return set_error(MIRAI_ERR_INVALID_ARG, "down_dx_rows_f32: null rank-block operand");
+  const RankBlock rb{rank_a, rank_b};
+  return run_f32<DXDOWN>("down_dx_rows_f32", grad_rows, offsets, num_sources, num_experts, num_rows, hidden, inter,
+                         grad_gate_up, const_cast<float*>(gate_up), w2, w2, hidden, inter, stream,
+                         rank_a ? &rb : nullptr, row_weights);
+}
+int mirai_moe_gateup_dx_f32(const void* grad_gate_up, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
+                            int64_t num_rows, int32_t inter, int32_t hidden, const void* w1, const void* w3,
+                            float* dx_sorted, mirai_stream_t stream) {
+  return run_f32<DXGATEUP>("gateup_dx_f32", grad_gate_up, offsets, num_sources, num_experts, num_rows, 2 * inter, hidden,
+                           dx_sorted, nullptr, w1, w3, inter, hidden, stream, nullptr, nullptr);
 }
 int mirai_moe_down_dx_lora_bf16(const void* grad_y, const int32_t* offsets, int32_t num_experts, int64_t num_rows,
                                 int32_t hidden, int32_t inter, const void* w2, const void* gate_up,

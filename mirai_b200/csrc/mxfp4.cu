@@ -398,7 +398,8 @@ struct Params {
   int a_bufs, b_stages;    // ring sizes
   int resident;            // 1: a row tile's A stays for the unit's whole run
   __nv_bfloat16* out;      // h [S, I] or y [S, H]; GATEUP: may be null when hq is wanted alone
-  __nv_bfloat16* gate_up;  // GATEUP: optional [S, 2I]
+  void* gate_up;           // GATEUP: optional [S, 2I] ...
+  int gate_up_f32;         // ... in bf16, or fp32
   uint8_t* hq;             // GATEUP: optional packed h [S, I/2] ...
   uint8_t* hscale;         // ... and its scale tiles
   int64_t h_blocks;        // row tiles of hscale
@@ -905,10 +906,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool valid = row < un.end;
       const bool boxed = __all_sync(0xffffffffu, valid);  // all 32 rows are the segment's
       const int row0 = (int)(row - lane);
-      // 32 rows x 32 columns: through the staging box and one TMA store, or row by row.  (A lane
+      // 32 rows x 32 bf16 columns (16 fp32 ones): through the staging box and one TMA store, or row by row.  (A lane
       // storing its own row straight to global memory touches 32 lines per store: 33 us more on the
       // 32768-token layer's gate/up.)
-      auto store = [&](const CUtensorMap* map, __nv_bfloat16* dst, int col, const uint32_t* w) {
+      auto store = [&](const CUtensorMap* map, void* dst, int col, const uint32_t* w) {
         if (boxed) {
           if (lane == 0) bulk_wait_group_read<0>();  // the box's previous store has read it
           __syncwarp();
@@ -953,8 +954,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int col = n * BM + c * 32;
             if (col >= p.N) break;  // warp-uniform
             uint32_t w[16];
-            if (p.gate_up) {
-              __nv_bfloat16* dst = p.gate_up + row * 2 * (int64_t)p.N + col;
+            if (p.gate_up && p.gate_up_f32) {
+              float* dst = static_cast<float*>(p.gate_up) + row * 2 * (int64_t)p.N + col;
+              store(&tmap_o1, dst, col, v[i]);
+              store(&tmap_o1, dst + 16, col + 16, v[i] + 16);
+              store(&tmap_o2, dst + p.N, col, v[i + 2]);
+              store(&tmap_o2, dst + p.N + 16, col + 16, v[i + 2] + 16);
+            } else if (p.gate_up) {
+              __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.gate_up) + row * 2 * (int64_t)p.N + col;
 #pragma unroll
               for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(v[i][2 * j]), __uint_as_float(v[i][2 * j + 1]));
               store(&tmap_o1, dst, col, w);
@@ -1048,7 +1055,8 @@ struct FewParams {
   int K, N;
   int n_tiles, w_blocks, stages;
   __nv_bfloat16* out;      // [S, N]
-  __nv_bfloat16* gate_up;  // GATEUP: optional [S, 2N]
+  void* gate_up;           // GATEUP: optional [S, 2N] in bf16, or fp32
+  int gate_up_f32;
 };
 
 struct alignas(16) FewSmem {
@@ -1342,8 +1350,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           if (MODE == GATEUP) {
             const float uv = __uint_as_float(up[i]);
             dst[(int64_t)i * p.N] = __float2bfloat16_rn(silu(gv) * uv);
-            if (p.gate_up) {
-              __nv_bfloat16* gu = p.gate_up + (int64_t)(tl.row + i) * 2 * p.N + ch;
+            if (p.gate_up && p.gate_up_f32) {
+              float* gu = static_cast<float*>(p.gate_up) + (int64_t)(tl.row + i) * 2 * p.N + ch;
+              gu[0] = gv;
+              gu[p.N] = uv;
+            } else if (p.gate_up) {
+              __nv_bfloat16* gu = static_cast<__nv_bfloat16*>(p.gate_up) + (int64_t)(tl.row + i) * 2 * p.N + ch;
               gu[0] = __float2bfloat16_rn(gv);
               gu[p.N] = __float2bfloat16_rn(uv);
             }
@@ -1379,7 +1391,10 @@ static int code_map(CUtensorMap& m, const uint8_t* packed, int64_t rows, int K) 
   return make_tmap_2d(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, (uint64_t)K / 2, (uint64_t)rows, (uint64_t)K / 2,
                       128, BM, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-static int out_map(CUtensorMap& m, void* out, int64_t rows, int N, int64_t ld) {
+static int out_map(CUtensorMap& m, void* out, int64_t rows, int N, int64_t ld, bool f32 = false) {
+  if (f32)
+    return make_tmap_2d(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, out, (uint64_t)N, (uint64_t)rows, (uint64_t)ld * 4, 16,
+                        32, CU_TENSOR_MAP_SWIZZLE_64B);
   return make_tmap_2d(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, (uint64_t)N, (uint64_t)rows, (uint64_t)ld * 2, 32,
                       32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
@@ -1437,7 +1452,8 @@ struct Operand {
 template <int MODE>
 static int product(const char* name, const Operand& a, const int32_t* offsets, int32_t nsrc, int32_t experts, int64_t S,
                    int32_t K, int32_t N, const mirai_mxfp4_weight* w0, const mirai_mxfp4_weight* w1, const void* rank_a,
-                   const void* rank_b, void* out, void* gate_up, uint8_t* hq, uint8_t* hscale, mirai_stream_t stream) {
+                   const void* rank_b, void* out, void* gate_up, int gate_up_dtype, uint8_t* hq, uint8_t* hscale,
+                   mirai_stream_t stream) {
   if (nsrc <= 0 || experts <= 0 || (int64_t)nsrc * experts > kMaxSegs)
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: %d sources x %d experts outside 1..%d segments", name, nsrc, experts,
                      kMaxSegs);
@@ -1452,6 +1468,9 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: null operand", name);
   if ((!out && !hq) || (hq && !hscale) || (!rank_a != !rank_b))
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: null output, scale or rank-block pointer", name);
+  if (gate_up_dtype != MIRAI_DTYPE_BF16 && gate_up_dtype != MIRAI_DTYPE_F32)
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: gate/up is saved in bf16 or fp32 (dtype %d)", name, gate_up_dtype);
+  const bool save_f32 = gate_up_dtype == MIRAI_DTYPE_F32;
   if (misaligned(out) || misaligned(gate_up) || misaligned(hq))
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: output not 16-byte aligned", name);
   const int kt = (int)ceil_div(K, 128);
@@ -1471,7 +1490,8 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   p.w_blocks = (int)ceil_div(N, kBlockRows);
   p.has_ext = rank_a != nullptr;
   p.out = static_cast<__nv_bfloat16*>(out);
-  p.gate_up = static_cast<__nv_bfloat16*>(gate_up);
+  p.gate_up = gate_up;
+  p.gate_up_f32 = save_f32;
   p.hq = hq;
   p.hscale = hscale;
   p.h_blocks = max_blocks(S, segs);
@@ -1496,8 +1516,8 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
   CUtensorMap to0 = ta, to1 = ta, to2 = ta;
   if (!rc && out) rc = out_map(to0, out, S, N, N);
   if (!rc && gate_up) {
-    rc = out_map(to1, gate_up, S, N, 2 * (int64_t)N);
-    if (!rc) rc = out_map(to2, static_cast<__nv_bfloat16*>(gate_up) + N, S, N, 2 * (int64_t)N);
+    rc = out_map(to1, gate_up, S, N, 2 * (int64_t)N, save_f32);
+    if (!rc) rc = out_map(to2, static_cast<char*>(gate_up) + (size_t)N * (save_f32 ? 4 : 2), S, N, 2 * (int64_t)N, save_f32);
   }
   if (rc) return rc;
   const int pairs_fit = resident_pairs<MODE>(name);
@@ -1538,7 +1558,7 @@ static int product(const char* name, const Operand& a, const int32_t* offsets, i
 template <int MODE>
 static int few_product(const char* name, const void* x, const int32_t* offsets, int32_t nsrc, int32_t experts, int64_t S,
                        int32_t K, int32_t N, const mirai_mxfp4_weight* w0, const mirai_mxfp4_weight* w1, void* out,
-                       void* gate_up, mirai_stream_t stream) {
+                       void* gate_up, int gate_up_dtype, mirai_stream_t stream) {
   if (nsrc <= 0 || experts <= 0 || (int64_t)nsrc * experts > kMaxSegs)
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: %d sources x %d experts outside 1..%d segments", name, nsrc, experts,
                      kMaxSegs);
@@ -1552,6 +1572,8 @@ static int few_product(const char* name, const void* x, const int32_t* offsets, 
   if (S == 0) return MIRAI_OK;
   if (!x || !offsets || !out || !w0 || !w0->packed || !w0->scale || (w1 && (!w1->packed || !w1->scale)))
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: null operand", name);
+  if (gate_up_dtype != MIRAI_DTYPE_BF16 && gate_up_dtype != MIRAI_DTYPE_F32)
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: gate/up is saved in bf16 or fp32 (dtype %d)", name, gate_up_dtype);
   if (misaligned(x, 32)) return set_error(MIRAI_ERR_INVALID_ARG, "%s: rows not 32-byte aligned", name);
   const int kt = (int)ceil_div(K, 128);
   FewParams p = {};
@@ -1565,7 +1587,8 @@ static int few_product(const char* name, const void* x, const int32_t* offsets, 
   p.n_tiles = (int)ceil_div(N, BM);
   p.w_blocks = p.n_tiles;
   p.out = static_cast<__nv_bfloat16*>(out);
-  p.gate_up = static_cast<__nv_bfloat16*>(gate_up);
+  p.gate_up = gate_up;
+  p.gate_up_f32 = gate_up_dtype == MIRAI_DTYPE_F32;
   p.stages = FEW_STAGES;
   while (few_smem_bytes<MODE>(p.stages, K, p.segs) > kSmemLimit) --p.stages;
   CUtensorMap t0, t1, s0, s1;
@@ -1691,28 +1714,46 @@ int mirai_mxfp4_quantize_rows(const void* x, int64_t x_rows, const int64_t* row_
   return check_launch("mxfp4_quantize_rows");
 }
 
+int mirai_moe_gateup_swiglu_mxfp4_save(const uint8_t* x_packed, const uint8_t* x_scale, const int32_t* offsets,
+                                       int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
+                                       int32_t inter, const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3,
+                                       void* h, void* gate_up, int32_t gate_up_dtype, uint8_t* h_packed,
+                                       uint8_t* h_scale, mirai_stream_t stream) {
+  if (!w3) return set_error(MIRAI_ERR_INVALID_ARG, "gateup_swiglu_mxfp4: null operand");
+  return mx::product<mx::GATEUP>("gateup_swiglu_mxfp4", {x_packed, x_scale}, offsets, num_sources, num_experts, num_rows,
+                                 hidden, inter, w1, w3, nullptr, nullptr, h, gate_up, gate_up_dtype, h_packed, h_scale,
+                                 stream);
+}
+
 int mirai_moe_gateup_swiglu_mxfp4(const uint8_t* x_packed, const uint8_t* x_scale, const int32_t* offsets,
                                   int32_t num_sources, int32_t num_experts, int64_t num_rows, int32_t hidden,
                                   int32_t inter, const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3, void* h,
                                   void* gate_up, uint8_t* h_packed, uint8_t* h_scale, mirai_stream_t stream) {
-  if (!w3) return set_error(MIRAI_ERR_INVALID_ARG, "gateup_swiglu_mxfp4: null operand");
-  return mx::product<mx::GATEUP>("gateup_swiglu_mxfp4", {x_packed, x_scale}, offsets, num_sources, num_experts, num_rows,
-                                 hidden, inter, w1, w3, nullptr, nullptr, h, gate_up, h_packed, h_scale, stream);
+  return mirai_moe_gateup_swiglu_mxfp4_save(x_packed, x_scale, offsets, num_sources, num_experts, num_rows, hidden, inter,
+                                            w1, w3, h, gate_up, MIRAI_DTYPE_BF16, h_packed, h_scale, stream);
+}
+
+int mirai_moe_gateup_swiglu_mxfp4_few_save(const void* x, const int32_t* offsets, int32_t num_sources,
+                                           int32_t num_experts, int64_t num_rows, int32_t hidden, int32_t inter,
+                                           const mirai_mxfp4_weight* w1, const mirai_mxfp4_weight* w3, void* h,
+                                           void* gate_up, int32_t gate_up_dtype, mirai_stream_t stream) {
+  if (!w3) return set_error(MIRAI_ERR_INVALID_ARG, "gateup_swiglu_mxfp4_few: null operand");
+  return mx::few_product<mx::GATEUP>("gateup_swiglu_mxfp4_few", x, offsets, num_sources, num_experts, num_rows, hidden,
+                                     inter, w1, w3, h, gate_up, gate_up_dtype, stream);
 }
 
 int mirai_moe_gateup_swiglu_mxfp4_few(const void* x, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
                                       int64_t num_rows, int32_t hidden, int32_t inter, const mirai_mxfp4_weight* w1,
                                       const mirai_mxfp4_weight* w3, void* h, void* gate_up, mirai_stream_t stream) {
-  if (!w3) return set_error(MIRAI_ERR_INVALID_ARG, "gateup_swiglu_mxfp4_few: null operand");
-  return mx::few_product<mx::GATEUP>("gateup_swiglu_mxfp4_few", x, offsets, num_sources, num_experts, num_rows, hidden,
-                                     inter, w1, w3, h, gate_up, stream);
+  return mirai_moe_gateup_swiglu_mxfp4_few_save(x, offsets, num_sources, num_experts, num_rows, hidden, inter, w1, w3, h,
+                                                gate_up, MIRAI_DTYPE_BF16, stream);
 }
 
 int mirai_moe_down_mxfp4_few(const void* h, const int32_t* offsets, int32_t num_sources, int32_t num_experts,
                              int64_t num_rows, int32_t inter, int32_t hidden, const mirai_mxfp4_weight* w2, void* y,
                              mirai_stream_t stream) {
   return mx::few_product<mx::DOWN>("down_mxfp4_few", h, offsets, num_sources, num_experts, num_rows, inter, hidden, w2,
-                                   nullptr, y, nullptr, stream);
+                                   nullptr, y, nullptr, MIRAI_DTYPE_BF16, stream);
 }
 
 int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const int32_t* offsets, int32_t num_sources,
@@ -1720,7 +1761,8 @@ int mirai_moe_down_mxfp4(const uint8_t* h_packed, const uint8_t* h_scale, const 
                          const mirai_mxfp4_weight* w2, const void* rank_a, const void* rank_b, void* y,
                          mirai_stream_t stream) {
   return mx::product<mx::DOWN>("down_mxfp4", {h_packed, h_scale}, offsets, num_sources, num_experts, num_rows, inter,
-                               hidden, w2, nullptr, rank_a, rank_b, y, nullptr, nullptr, nullptr, stream);
+                               hidden, w2, nullptr, rank_a, rank_b, y, nullptr, MIRAI_DTYPE_BF16, nullptr, nullptr,
+                               stream);
 }
 
 }  // extern "C"

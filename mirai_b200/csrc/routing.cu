@@ -312,6 +312,8 @@ constexpr int kMaxTopK = 16;
 
 __device__ __forceinline__ float bf16r_(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
+// F32: the rows are fp32 (two 16-byte words for the 8 columns one holds in bf16).
+template <bool F32>
 __global__ void __launch_bounds__(256) combine_kernel(const uint4* __restrict__ y, const int64_t* __restrict__ inv,
                                                       const float* __restrict__ w, int64_t T, int k, int H,
                                                       int64_t S, void* __restrict__ out, int out_dtype) {
@@ -347,6 +349,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const uint4* __restrict__ 
 #pragma unroll
     for (int q = 0; q < 8; ++q) acc[q] = 0.f;
     for (int j = 0; j < k; ++j) {
+      if constexpr (F32) {
+        const float4* row = reinterpret_cast<const float4*>(y) + (pos[j] * vec_per_row + v) * 2;
+        const float4 a = __ldg(row), b = __ldg(row + 1);
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] = __fadd_rn(acc[q], __fmul_rn(x[q], wt[j]));
+        continue;
+      }
       const uint4 u = __ldg(y + pos[j] * vec_per_row + v);
       const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
       if (out_dtype == MIRAI_COMBINE_BF16_ACCUM) {
@@ -383,12 +393,15 @@ __global__ void __launch_bounds__(256) combine_kernel(const uint4* __restrict__ 
 // ============================================================================
 // a8 backward: one warp per token.  grad_y rows are written in place of the
 // token's routes; the score gradient is an fp32 dot product per route.
+// ROWS: the rows are the output's gradient as it came (exact), and the routing
+// weights go beside them, fp32 [S], for the product that multiplies by them in fp32.
 // ============================================================================
+template <bool ROWS>
 __global__ void __launch_bounds__(256) combine_backward_kernel(const uint4* __restrict__ g, const uint4* __restrict__ y,
                                                                const int64_t* __restrict__ inv,
                                                                const float* __restrict__ w, int64_t T, int k, int H,
                                                                int64_t S, uint4* __restrict__ gy,
-                                                               float* __restrict__ gw) {
+                                                               float* __restrict__ gw, float* __restrict__ row_w) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
   if (t >= T) return;
@@ -412,13 +425,16 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const uint4* __re
         const float g0 = bf16_lo(gw4[q]), g1 = bf16_hi(gw4[q]);
         dot = fmaf(g0, bf16_lo(yw4[q]), dot);
         dot = fmaf(g1, bf16_hi(yw4[q]), dot);
-        o[q] = pack_bf16x2(g0 * wt, g1 * wt);
+        o[q] = ROWS ? gw4[q] : pack_bf16x2(g0 * wt, g1 * wt);
       }
       gy[pos * vec_per_row + v] = make_uint4(o[0], o[1], o[2], o[3]);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    if (lane == 0) gw[t * k + j] = dot;
+    if (lane == 0) {
+      gw[t * k + j] = dot;
+      if (ROWS) row_w[pos] = wt;
+    }
   }
 }
 
@@ -536,37 +552,71 @@ int mirai_permute_rows_bf16(const void* tokens, int64_t num_tokens, const int64_
   return check_launch("permute_rows");
 }
 
+static int combine_impl(const char* name, bool f32, const void* y_sorted, const int64_t* inverse_order,
+                        const float* top_weights, int64_t num_tokens, int32_t top_k, int32_t hidden, void* out,
+                        int32_t out_dtype, mirai_stream_t stream) {
+  if (num_tokens < 0 || top_k <= 0 || top_k > kMaxTopK || hidden <= 0 || hidden % 8 != 0)
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: need 0 < k <= %d and hidden %% 8 == 0", name, kMaxTopK);
+  if (out_dtype != MIRAI_DTYPE_BF16 && out_dtype != MIRAI_DTYPE_F32 &&
+      (f32 || out_dtype != MIRAI_COMBINE_BF16_ACCUM))
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: unknown out_dtype %d", name, out_dtype);
+  if (num_tokens == 0) return MIRAI_OK;
+  if (!y_sorted || !inverse_order || !out || misaligned16(y_sorted) || misaligned16(out))
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: null or misaligned pointer", name);
+  const int blocks = (int)((num_tokens + 7) / 8);
+  auto* kernel = f32 ? combine_kernel<true> : combine_kernel<false>;
+  kernel<<<blocks, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint4*>(y_sorted), inverse_order, top_weights, num_tokens, top_k, hidden,
+      num_tokens * top_k, out, out_dtype);
+  return check_launch(name);
+}
+
 int mirai_moe_combine(const void* y_sorted, const int64_t* inverse_order, const float* top_weights,
                       int64_t num_tokens, int32_t top_k, int32_t hidden, void* out, int32_t out_dtype,
                       mirai_stream_t stream) {
+  return combine_impl("combine", false, y_sorted, inverse_order, top_weights, num_tokens, top_k, hidden, out, out_dtype,
+                      stream);
+}
+
+int mirai_moe_combine_f32(const float* y_sorted, const int64_t* inverse_order, const float* top_weights,
+                          int64_t num_tokens, int32_t top_k, int32_t hidden, void* out, int32_t out_dtype,
+                          mirai_stream_t stream) {
+  return combine_impl("combine_f32", true, y_sorted, inverse_order, top_weights, num_tokens, top_k, hidden, out,
+                      out_dtype, stream);
+}
+
+static int combine_backward_impl(const char* name, const void* grad_out, const void* y_sorted,
+                                 const int64_t* inverse_order, const float* top_weights, int64_t num_tokens,
+                                 int32_t top_k, int32_t hidden, void* grad_y_sorted, float* row_weights,
+                                 float* grad_weights, mirai_stream_t stream) {
   if (num_tokens < 0 || top_k <= 0 || top_k > kMaxTopK || hidden <= 0 || hidden % 8 != 0)
-    return set_error(MIRAI_ERR_INVALID_ARG, "combine: need 0 < k <= %d and hidden %% 8 == 0", kMaxTopK);
-  if (out_dtype != MIRAI_DTYPE_BF16 && out_dtype != MIRAI_DTYPE_F32 && out_dtype != MIRAI_COMBINE_BF16_ACCUM)
-    return set_error(MIRAI_ERR_INVALID_ARG, "combine: unknown out_dtype %d", out_dtype);
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: need 0 < k <= %d and hidden %% 8 == 0", name, kMaxTopK);
   if (num_tokens == 0) return MIRAI_OK;
-  if (!y_sorted || !inverse_order || !out || misaligned16(y_sorted) || misaligned16(out))
-    return set_error(MIRAI_ERR_INVALID_ARG, "combine: null or misaligned pointer");
+  if (!grad_out || !y_sorted || !inverse_order || !top_weights || !grad_y_sorted || !grad_weights ||
+      misaligned16(grad_out) || misaligned16(y_sorted) || misaligned16(grad_y_sorted))
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: null or misaligned pointer", name);
   const int blocks = (int)((num_tokens + 7) / 8);
-  combine_kernel<<<blocks, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint4*>(y_sorted), inverse_order, top_weights, num_tokens, top_k, hidden,
-      num_tokens * top_k, out, out_dtype);
-  return check_launch("combine");
+  auto* kernel = row_weights ? combine_backward_kernel<true> : combine_backward_kernel<false>;
+  kernel<<<blocks, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint4*>(grad_out), static_cast<const uint4*>(y_sorted), inverse_order, top_weights,
+      num_tokens, top_k, hidden, num_tokens * top_k, static_cast<uint4*>(grad_y_sorted), grad_weights, row_weights);
+  return check_launch(name);
 }
 
 int mirai_moe_combine_backward(const void* grad_out, const void* y_sorted, const int64_t* inverse_order,
                                const float* top_weights, int64_t num_tokens, int32_t top_k, int32_t hidden,
                                void* grad_y_sorted, float* grad_weights, mirai_stream_t stream) {
-  if (num_tokens < 0 || top_k <= 0 || top_k > kMaxTopK || hidden <= 0 || hidden % 8 != 0)
-    return set_error(MIRAI_ERR_INVALID_ARG, "combine_backward: need 0 < k <= %d and hidden %% 8 == 0", kMaxTopK);
-  if (num_tokens == 0) return MIRAI_OK;
-  if (!grad_out || !y_sorted || !inverse_order || !top_weights || !grad_y_sorted || !grad_weights ||
-      misaligned16(grad_out) || misaligned16(y_sorted) || misaligned16(grad_y_sorted))
-    return set_error(MIRAI_ERR_INVALID_ARG, "combine_backward: null or misaligned pointer");
-  const int blocks = (int)((num_tokens + 7) / 8);
-  combine_backward_kernel<<<blocks, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint4*>(grad_out), static_cast<const uint4*>(y_sorted), inverse_order, top_weights,
-      num_tokens, top_k, hidden, num_tokens * top_k, static_cast<uint4*>(grad_y_sorted), grad_weights);
-  return check_launch("combine_backward");
+  return combine_backward_impl("combine_backward", grad_out, y_sorted, inverse_order, top_weights, num_tokens, top_k,
+                               hidden, grad_y_sorted, nullptr, grad_weights, stream);
+}
+
+int mirai_moe_combine_backward_rows(const void* grad_out, const void* y_sorted, const int64_t* inverse_order,
+                                    const float* top_weights, int64_t num_tokens, int32_t top_k, int32_t hidden,
+                                    void* grad_rows, float* row_weights, float* grad_weights, mirai_stream_t stream) {
+  if (num_tokens > 0 && !row_weights)
+    return set_error(MIRAI_ERR_INVALID_ARG, "combine_backward_rows: null pointer");
+  return combine_backward_impl("combine_backward_rows", grad_out, y_sorted, inverse_order, top_weights, num_tokens,
+                               top_k, hidden, grad_rows, row_weights, grad_weights, stream);
 }
 
 }  // extern "C"

@@ -565,8 +565,12 @@ def _mxfp4_output(out: torch.Tensor | None, shape: tuple, device) -> torch.Tenso
 
 
 def _gateup_mxfp4(x, offsets: torch.Tensor, w1: Mxfp4Tensor, w3: Mxfp4Tensor, *, inter: int, save_gate_up: bool,
-                  want_h: bool, want_rows: bool, out: torch.Tensor | None = None, sources: int = 1):
+                  want_h: bool, want_rows: bool, out: torch.Tensor | None = None, sources: int = 1,
+                  gate_up_dtype: torch.dtype = torch.bfloat16):
     """(h or None, gate_up or None, quantised h or None)."""
+    if gate_up_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"gate/up is saved in bf16 or fp32, not {gate_up_dtype}")
+    save_code = _MXFP4_DTYPES[gate_up_dtype]
     if not isinstance(w1, Mxfp4Tensor) or not isinstance(w3, Mxfp4Tensor) or w1.shape != w3.shape:
         raise TypeError("gate/up in MXFP4 needs two Mxfp4Tensor keys of one shape")
     E, out_f, hidden = w1.shape
@@ -580,18 +584,18 @@ def _gateup_mxfp4(x, offsets: torch.Tensor, w1: Mxfp4Tensor, w3: Mxfp4Tensor, *,
         x = _few_input(x, hidden, "x_sorted")
         S = x.shape[0]
         h = _mxfp4_output(out, (S, inter), device)
-        gu = torch.empty((S, 2 * inter), dtype=torch.bfloat16, device=device) if save_gate_up else None
-        _run(device, "mirai_moe_gateup_swiglu_mxfp4_few", x.data_ptr(), offsets.data_ptr(), sources, E, S, hidden, inter,
-             w1.struct(), w3.struct(), h.data_ptr(), None if gu is None else gu.data_ptr())
+        gu = torch.empty((S, 2 * inter), dtype=gate_up_dtype, device=device) if save_gate_up else None
+        _run(device, "mirai_moe_gateup_swiglu_mxfp4_few_save", x.data_ptr(), offsets.data_ptr(), sources, E, S, hidden,
+             inter, w1.struct(), w3.struct(), h.data_ptr(), None if gu is None else gu.data_ptr(), save_code)
         return h, gu, None
     rows = _mxfp4_rows(x, offsets, hidden, "x_sorted")
     S = rows.shape[0]
     h = _mxfp4_output(out, (S, inter), device) if want_h else None
-    gu = torch.empty((S, 2 * inter), dtype=torch.bfloat16, device=device) if save_gate_up else None
+    gu = torch.empty((S, 2 * inter), dtype=gate_up_dtype, device=device) if save_gate_up else None
     hq = Mxfp4Rows.empty(S, inter, offsets.numel(), device) if want_rows else None
-    _run(device, "mirai_moe_gateup_swiglu_mxfp4", rows.packed.data_ptr(), rows.scale.data_ptr(), offsets.data_ptr(),
+    _run(device, "mirai_moe_gateup_swiglu_mxfp4_save", rows.packed.data_ptr(), rows.scale.data_ptr(), offsets.data_ptr(),
          sources, E, S, hidden, inter, w1.struct(), w3.struct(), None if h is None else h.data_ptr(),
-         None if gu is None else gu.data_ptr(), None if hq is None else hq.packed.data_ptr(),
+         None if gu is None else gu.data_ptr(), save_code, None if hq is None else hq.packed.data_ptr(),
          None if hq is None else hq.scale.data_ptr())
     return h, gu, hq
 
@@ -651,7 +655,7 @@ def _as_weight(w):
 
 def gateup_swiglu(x_sorted: torch.Tensor, offsets: torch.Tensor, w1, w3, *, inter: int,
                   save_gate_up: bool = False, out: torch.Tensor | None = None, sources: int = 1,
-                  quantize: bool = False):
+                  quantize: bool = False, gate_up_dtype: torch.dtype = torch.bfloat16):
     """h = silu(x W1^T) * (x W3^T) per expert segment.  ``w1``/``w3`` are bf16
     tensors [E, I, H], or ``Nf4Weight`` / ``Int8Weight`` descriptors.
     ``sources`` > 1: ``offsets`` ends ``sources * E`` source-major segments
@@ -660,16 +664,20 @@ def gateup_swiglu(x_sorted: torch.Tensor, offsets: torch.Tensor, w1, w3, *, inte
     ``Mxfp4Tensor`` keys multiply the rows in MXFP4 too: ``x_sorted`` is bf16
     (quantised here) or ``Mxfp4Rows``; silu(g) * u is formed in fp32 and rounded
     once, and ``quantize=True`` returns h as the ``Mxfp4Rows`` that ``down``
-    takes instead of bf16."""
+    takes instead of bf16.  ``gate_up_dtype=torch.float32`` saves the gate/up
+    accumulators themselves, which ``down_dx`` takes as well."""
     if isinstance(w1, Mxfp4Tensor) or isinstance(w3, Mxfp4Tensor):
         if quantize and out is not None:
             raise ValueError("quantize=True returns Mxfp4Rows: it writes no bf16 out")
         h, gu, hq = _gateup_mxfp4(x_sorted, offsets, w1, w3, inter=inter, save_gate_up=save_gate_up,
-                                  want_h=not quantize, want_rows=quantize, out=out, sources=sources)
+                                  want_h=not quantize, want_rows=quantize, out=out, sources=sources,
+                                  gate_up_dtype=gate_up_dtype)
         h = hq if quantize else h
         return (h, gu) if save_gate_up else h
     if quantize:
         raise TypeError("quantize=True needs MXFP4 keys")
+    if gate_up_dtype != torch.bfloat16:
+        raise TypeError(f"gate/up saved in {gate_up_dtype} needs MXFP4 keys")
     w1, w3 = _as_weight(w1), _as_weight(w3)
     x_sorted = _cuda(x_sorted, "x_sorted", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
@@ -831,8 +839,12 @@ def combine(y_sorted: torch.Tensor, inverse_order: torch.Tensor, top_weights: to
             top_k: int | None = None, bf16_accumulate: bool = False) -> torch.Tensor:
     """Weighted un-permute; ``top_weights=None`` sums the routes (permute backward).
     ``bf16_accumulate``: bf16 products summed in bf16, route by route (MAGI-2's
-    index_add on bf16 tensors) instead of one fp32 sum."""
-    y_sorted = _cuda(y_sorted, "y_sorted", torch.bfloat16)
+    index_add on bf16 tensors) instead of one fp32 sum.  ``y_sorted`` is bf16 or
+    fp32 (summed in fp32)."""
+    y_sorted = _cuda(y_sorted, "y_sorted")
+    rows_f32 = y_sorted.dtype == torch.float32
+    if not rows_f32 and y_sorted.dtype != torch.bfloat16 or rows_f32 and bf16_accumulate:
+        raise TypeError(f"y_sorted must be torch.bfloat16 (or fp32 without bf16_accumulate), got {y_sorted.dtype}")
     inv = _cuda(inverse_order, "inverse_order", torch.int64)
     if top_weights is None:
         k = int(top_k)
@@ -849,7 +861,8 @@ def combine(y_sorted: torch.Tensor, inverse_order: torch.Tensor, top_weights: to
         if out.dtype != torch.bfloat16:
             raise TypeError("bf16 accumulation writes a bf16 output")
         code = COMBINE_BF16_ACCUM
-    _lib.call("mirai_moe_combine", _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H, _ptr(out), code, _stream())
+    _lib.call("mirai_moe_combine_f32" if rows_f32 else "mirai_moe_combine", _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H,
+              _ptr(out), code, _stream())
     return out
 
 
@@ -867,6 +880,28 @@ def combine_backward(grad_out: torch.Tensor, y_sorted: torch.Tensor, inverse_ord
     _lib.call("mirai_moe_combine_backward", _ptr(g), _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H, _ptr(gy),
               _ptr(gw), _stream())
     return gy, gw
+
+
+def combine_backward_rows(grad_out: torch.Tensor, y_sorted: torch.Tensor, inverse_order: torch.Tensor,
+                          top_weights: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``combine_backward`` without its rounding: (grad_rows bf16 [S, H], each route's row of
+    ``grad_out`` as it is, row_weights fp32 [S], grad_weights fp32 [T, k]); grad_y_sorted is
+    grad_rows * row_weights[:, None]."""
+    g = _cuda(grad_out.to(torch.bfloat16), "grad_out", torch.bfloat16)
+    y_sorted = _cuda(y_sorted, "y_sorted", torch.bfloat16)
+    inv = _cuda(inverse_order, "inverse_order", torch.int64)
+    w = _cuda(top_weights.float(), "top_weights", torch.float32)
+    T, k = w.shape
+    H = y_sorted.shape[1]
+    if tuple(g.shape) != (T, H) or y_sorted.shape[0] != T * k or inv.numel() != T * k:
+        raise ValueError(f"grad_out {tuple(g.shape)}, rows {tuple(y_sorted.shape)} and {inv.numel()} routes do not fit "
+                         f"weights {tuple(w.shape)}")
+    rows = torch.empty_like(y_sorted)
+    rw = torch.empty(T * k, dtype=torch.float32, device=g.device)
+    gw = torch.empty((T, k), dtype=torch.float32, device=g.device)
+    _lib.call("mirai_moe_combine_backward_rows", _ptr(g), _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H, _ptr(rows),
+              _ptr(rw), _ptr(gw), _stream())
+    return rows, rw, gw
 
 
 # ----------------------------------------------------------------------------- a9 dX
@@ -891,7 +926,8 @@ def down_dx(grad_y: torch.Tensor, offsets: torch.Tensor, w2, gate_up: torch.Tens
     """grad_gate_up [S, 2I] = SwiGLU backward of (gate, up) given dh = grad_y W2
     (+ the LoRA path's input gradient when ``lora``).  ``sources`` > 1:
     source-major segments (an expert owner's rows); there ``gate_up=None``
-    returns dh [S, I] itself."""
+    returns dh [S, I] itself.  An ``Mxfp4Tensor`` key takes ``gate_up`` in bf16
+    or fp32 (and needs it)."""
     if isinstance(w2, Mxfp4Tensor):
         return _down_dx_mxfp4(grad_y, offsets, w2, gate_up, inter=inter, out=out, lora=lora, rank_a=rank_a,
                               sources=sources)
@@ -930,12 +966,16 @@ def down_dx(grad_y: torch.Tensor, offsets: torch.Tensor, w2, gate_up: torch.Tens
 
 
 def _down_dx_mxfp4(grad_y, offsets, w2: Mxfp4Tensor, gate_up, *, inter: int, out, lora, rank_a, sources: int,
-                   dense: torch.Tensor | None = None) -> torch.Tensor:
+                   dense: torch.Tensor | None = None, row_weights: torch.Tensor | None = None) -> torch.Tensor:
     """``down_dx`` on an MXFP4 key: its read-back values (``dense`` when the caller has
-    them), the SwiGLU backward in fp32 as the forward's."""
+    them), the SwiGLU backward in fp32 as the forward's.  ``row_weights`` fp32 [S] (with
+    gate/up in fp32): dh is multiplied by them, as ``combine_backward_rows`` leaves it to do."""
     gy = _cuda(grad_y, "grad_y", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
-    gu = _cuda(gate_up, "gate_up", torch.bfloat16)  # (no dh alone: the MXFP4 forward saves gate/up)
+    gu = _cuda(gate_up, "gate_up")  # (no dh alone: the MXFP4 forward saves gate/up)
+    wide = gu.dtype == torch.float32
+    if not wide and (gu.dtype != torch.bfloat16 or row_weights is not None):
+        raise TypeError(f"gate_up must be bf16 or fp32 (fp32 with row weights), got {gu.dtype}")
     E, hidden, key_inter = w2.shape
     S = gy.shape[0]
     if gy.shape != (S, hidden) or key_inter != inter or gu.shape != (S, 2 * inter) or offsets.numel() != sources * E:
@@ -948,6 +988,11 @@ def _down_dx_mxfp4(grad_y, offsets, w2: Mxfp4Tensor, gate_up, *, inter: int, out
         low = rank_a if rank_a is not None else lora_project(gy, offsets, lora, forward=False, sources=sources)
         rank_b = lora.a_pad()
     dgu = _mxfp4_output(out, (S, 2 * inter), w2.device)
+    if wide:
+        _run(w2.device, "mirai_moe_down_dx_rows_f32", gy.data_ptr(), _ptr(row_weights), offsets.data_ptr(), sources, E, S,
+             hidden, inter, w.data_ptr(), gu.data_ptr(), None if low is None else low.data_ptr(),
+             None if rank_b is None else rank_b.data_ptr(), dgu.data_ptr())
+        return dgu
     _run(w2.device, "mirai_moe_down_dx_f32_bf16", gy.data_ptr(), offsets.data_ptr(), sources, E, S, hidden, inter,
          w.data_ptr(), gu.data_ptr(), None if low is None else low.data_ptr(),
          None if rank_b is None else rank_b.data_ptr(), dgu.data_ptr())
@@ -993,13 +1038,18 @@ def lora_grad(x: torch.Tensor, g_rank: torch.Tensor, offsets: torch.Tensor, rank
 
 
 def gateup_dx(grad_gate_up: torch.Tensor, offsets: torch.Tensor, w1, w3, *, hidden: int,
-              out: torch.Tensor | None = None, sources: int = 1) -> torch.Tensor:
+              out: torch.Tensor | None = None, sources: int = 1, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """dx_sorted [S, H] = dgate W1 + dup W3 per expert segment (``sources`` > 1:
-    source-major segments)."""
+    source-major segments).  ``out_dtype=torch.float32`` (bf16 or MXFP4 keys):
+    the accumulator unrounded."""
     w1, w3 = _as_weight(_dx_weight(w1)), _as_weight(_dx_weight(w3))
     dgu = _cuda(grad_gate_up, "grad_gate_up", torch.bfloat16)
     offsets = _cuda(offsets, "offsets", torch.int32)
     S, I2 = dgu.shape
+    if out_dtype == torch.float32:
+        return _gateup_dx_f32(dgu, offsets, w1, w3, hidden=hidden, out=out, sources=sources)
+    if out_dtype != torch.bfloat16:
+        raise TypeError(f"dx_sorted is bf16 or fp32, not {out_dtype}")
     dxs = out if out is not None else torch.empty((S, hidden), dtype=torch.bfloat16, device=dgu.device)
     if sources > 1:
         if offsets.numel() % sources:
@@ -1010,6 +1060,28 @@ def gateup_dx(grad_gate_up: torch.Tensor, offsets: torch.Tensor, w1, w3, *, hidd
     _lib.call(f"mirai_moe_gateup_dx_{_fmt_suffix(w1)}", _ptr(dgu), _ptr(offsets), offsets.numel(), S, I2 // 2,
               hidden, _wptr(w1), _wptr(w3), _ptr(dxs), _stream())
     return dxs
+
+
+def _gateup_dx_f32(dgu: torch.Tensor, offsets: torch.Tensor, w1, w3, *, hidden: int, out: torch.Tensor | None,
+                   sources: int) -> torch.Tensor:
+    if not isinstance(w1, torch.Tensor) or not isinstance(w3, torch.Tensor):
+        raise TypeError("dx_sorted in fp32 needs bf16 or MXFP4 keys")
+    w1, w3 = _cuda(w1, "w1", torch.bfloat16), _cuda(w3, "w3", torch.bfloat16)
+    S, I2 = dgu.shape
+    E = w1.shape[0]
+    if tuple(w1.shape) != (E, I2 // 2, hidden) or w3.shape != w1.shape or offsets.numel() != sources * E:
+        raise ValueError(f"keys {tuple(w1.shape)} and {tuple(w3.shape)} with {offsets.numel()} segments of {sources} "
+                         f"source(s): the call has inter {I2 // 2} and hidden {hidden}")
+    _same_device(dgu.device, offsets=offsets, w1=w1, w3=w3)
+    if out is None:
+        out = torch.empty((S, hidden), dtype=torch.float32, device=dgu.device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (S, hidden) or not out.is_contiguous() \
+            or out.device != dgu.device:
+        raise ValueError(f"out must be a contiguous fp32 {(S, hidden)} tensor on {dgu.device}, got {out.dtype} "
+                         f"{tuple(out.shape)} on {out.device}")
+    _run(dgu.device, "mirai_moe_gateup_dx_f32", dgu.data_ptr(), offsets.data_ptr(), sources, E, S, I2 // 2, hidden,
+         w1.data_ptr(), w3.data_ptr(), out.data_ptr())
+    return out
 
 
 # ----------------------------------------------------------------------------- any layout / activation / group count
@@ -1109,17 +1181,18 @@ def moe_forward(tokens: torch.Tensor, top_indices: torch.Tensor, top_weights: to
 def _mxfp4_experts(tokens, plan: DispatchPlan, w1, w3, w2, *, inter: int, lora: DownLoRA | None, train: bool):
     """(y, gate_up, h, rank_a) of the routed rows in MXFP4: quantised in the
     permute's pass, h in the gate/up epilogue (a generation step's few rows inside
-    the products).  gate_up when ``train``; h and rank_a with a LoRA adapter,
+    the products).  gate_up (fp32) when ``train``; h and rank_a with a LoRA adapter,
     whose projection reads h in bf16."""
     if not all(isinstance(w, Mxfp4Tensor) for w in (w1, w3, w2)):
         raise TypeError("MXFP4 experts hold all three keys in MXFP4")
     if lora is None and plan.total_slots <= _few_limit(plan.offsets.numel()) and max(tokens.shape[1], inter) <= _FEW_MAX_WIDTH:
         rows = permute_rows(tokens, plan.sorted_token_indices)
-        h, gu, _ = _gateup_mxfp4(rows, plan.offsets, w1, w3, inter=inter, save_gate_up=train, want_h=True, want_rows=False)
+        h, gu, _ = _gateup_mxfp4(rows, plan.offsets, w1, w3, inter=inter, save_gate_up=train, want_h=True, want_rows=False,
+                                 gate_up_dtype=torch.float32)
         return down(h, plan.offsets, w2, hidden=tokens.shape[1]), gu, None, None
     rows = mxfp4_quantize_rows(tokens, plan.offsets, row_index=plan.sorted_token_indices)
     h, gu, hq = _gateup_mxfp4(rows, plan.offsets, w1, w3, inter=inter, save_gate_up=train, want_h=lora is not None,
-                              want_rows=True)
+                              want_rows=True, gate_up_dtype=torch.float32)
     low = lora_project(h, plan.offsets, lora, forward=True) if lora is not None else None
     return down(hq, plan.offsets, w2, hidden=tokens.shape[1], lora=lora, rank_a=low), gu, h, low
 
@@ -1130,7 +1203,7 @@ class ForwardState:
 
     plan: DispatchPlan
     y_sorted: torch.Tensor   # [S, H] bf16 expert outputs
-    gate_up: torch.Tensor    # [S, 2I] bf16 saved pre-activations
+    gate_up: torch.Tensor    # [S, 2I] saved pre-activations, bf16 (an MXFP4 layer's: fp32)
     top_weights: torch.Tensor
     h: torch.Tensor | None = None         # [S, I] bf16, kept when LoRA factor grads are wanted
     rank_a: torch.Tensor | None = None    # [S, 64] LoRA rank block of h (scaled)
@@ -1263,6 +1336,38 @@ def moe_forward_train(tokens, top_indices, top_weights, w1, w3, w2, *, num_exper
     return out, ForwardState(plan, y, gu, top_weights.float(), h if keep else None, low if keep else None, staged)
 
 
+def _mxfp4_backward(grad_out, state: ForwardState, w1, w3, w2, *, inter: int, out_dtype: torch.dtype,
+                    lora: DownLoRA | None):
+    """``moe_backward_dx`` on MXFP4 keys.  The stored values are read back to bf16, w2
+    first, beside the combine backward and the down dX.  dx is rounded where an MMA
+    operand must be bf16 (dgate / dup) and at the end; the rows that go into the down
+    dX are the output's gradient itself, weighted in its epilogue, and gate/up and the
+    routes' dx stay in fp32."""
+    plan, H = state.plan, state.y_sorted.shape[1]
+    dense, join = _read_back_beside((w2, w1, w3))
+    rows, rw, gw = combine_backward_rows(grad_out, state.y_sorted, plan.inverse_order, state.top_weights)
+    glow = None
+    if lora is not None:
+        E, Hb, r = lora.b.shape
+        glow = lora_project(rows, plan.offsets, lora, forward=False)
+        if lora.compute_grads:
+            if state.h is None or state.rank_a is None:
+                raise RuntimeError("LoRA factor gradients need the forward run with compute_grads=True")
+            Ia = lora.a.shape[2]
+            # the [S, 64] operand of each sum over rows takes the rows' weights
+            weighted = [(t * rw[:, None]).to(torch.bfloat16) for t in (glow, state.rank_a)]
+            lora.grad_a = lora_grad(state.h, weighted[0], plan.offsets, r,
+                                    torch.empty((E, r, Ia), dtype=torch.float32, device=rows.device), (r * Ia, Ia, 1))
+            lora.grad_b = lora_grad(rows, weighted[1], plan.offsets, r,
+                                    torch.empty((E, Hb, r), dtype=torch.float32, device=rows.device), (Hb * r, 1, r))
+    join(1)
+    dgu = _down_dx_mxfp4(rows, plan.offsets, w2, state.gate_up, inter=inter, out=None, lora=lora, rank_a=glow, sources=1,
+                         dense=dense[0], row_weights=rw)
+    join(3)
+    dxs = _gateup_dx_f32(dgu, plan.offsets, dense[1], dense[2], hidden=H, out=None, sources=1)
+    return combine(dxs, plan.inverse_order, None, out_dtype=out_dtype, top_k=plan.top_k), gw
+
+
 def moe_backward_dx(grad_out: torch.Tensor, state: ForwardState, w1, w3, w2, *, inter: int,
                     out_dtype: torch.dtype = torch.bfloat16, lora: DownLoRA | None = None):
     """Input gradient through the frozen experts and the top-weight gradient.
@@ -1270,10 +1375,9 @@ def moe_backward_dx(grad_out: torch.Tensor, state: ForwardState, w1, w3, w2, *, 
     grad_out [T, H] -> (dx [T, H], d_top_weights fp32 [T, k])."""
     plan = state.plan
     H = state.y_sorted.shape[1]
-    mx = isinstance(w2, Mxfp4Tensor)
-    if mx:  # the stored values in bf16, w2 first, beside the combine backward and the down dX
-        dense, join = _read_back_beside((w2, w1, w3))
-    elif state.staged is not None and all(a is b for a, b in zip(state.staged[0], (w1, w3, w2))):
+    if isinstance(w2, Mxfp4Tensor):
+        return _mxfp4_backward(grad_out, state, w1, w3, w2, inter=inter, out_dtype=out_dtype, lora=lora)
+    if state.staged is not None and all(a is b for a, b in zip(state.staged[0], (w1, w3, w2))):
         w1, w3, w2 = state.staged[1]  # the forward's bf16 copies of these NF4 keys
         state.staged = None
     else:
@@ -1291,13 +1395,6 @@ def moe_backward_dx(grad_out: torch.Tensor, state: ForwardState, w1, w3, w2, *, 
                                     torch.empty((E, r, Ia), dtype=torch.float32, device=gy.device), (r * Ia, Ia, 1))
             lora.grad_b = lora_grad(gy, state.rank_a, plan.offsets, r,
                                     torch.empty((E, Hb, r), dtype=torch.float32, device=gy.device), (Hb * r, 1, r))
-    if mx:
-        join(1)
-        dgu = _down_dx_mxfp4(gy, plan.offsets, w2, state.gate_up, inter=inter, out=None, lora=lora, rank_a=glow, sources=1,
-                             dense=dense[0])
-        join(3)
-        dxs = gateup_dx(dgu, plan.offsets, dense[1], dense[2], hidden=H)
-        return combine(dxs, plan.inverse_order, None, out_dtype=out_dtype, top_k=plan.top_k), gw
     g_in, g_mid = _rotations(w1, w3, w2)
     if g_mid:  # rotated INT8: dh = rotate(grad_y (q s)), then the SwiGLU backward
         dh = down_dh(gy, plan.offsets, w2, inter=inter, lora=lora, rank_a=glow)
