@@ -459,9 +459,14 @@ __global__ void __launch_bounds__(256, PER <= 16 ? 4 : (PER <= 32 ? 2 : 1))
 }
 
 // ----------------------------------------------------------------------------
-// Backward: dL/ds_j = scale (g_j - [den follows] sum_i g_i s_i / den) / den, then
-//   sigmoid  dl_e = ds s (1 - s) at the selected experts, 0 elsewhere
-//   softmax  dl_e = s_e (ds_e - sum_j ds_j s_j)
+// Backward: dL/ds_j = scale a_j / den, a_j = g_j, or where den follows the scores' sum
+// (den = sum + eps)  a_j = g_j - sum_i g_i s_i / den = sum_i (g_j - g_i) s_i / den + g_j eps / den;
+//   sigmoid  dl_e = ds_e s (1 - s) at the selected experts, 0 elsewhere
+//   softmax  dl_e = s_e (ds_e - sum_j ds_j s_j), the sum being scale sum_j g_j s_j / den, times
+//            eps / den where den follows
+// One score near 1 (a sure router) leaves nothing of a difference of rounded scores, so none is
+// formed: 1 - s is the sigmoid of -l, or the other experts' share of the softmax, a_j is summed from
+// differences of the gradients, and ds_e - sum_j ds_j s_j (den fixed) is g_e (1 - s_e) less the others' g s.
 // W lanes per token (a warp takes 32 / W, since one token's chain of dependent loads is
 // latency): the row is streamed once (softmax) and its gradient written once, zeros or the
 // softmax tail everywhere, then slot j's lane corrects its expert (an index given twice
@@ -510,6 +515,7 @@ __global__ void __launch_bounds__(256) route_groups_backward_kernel(const float*
   }
   float l[PER];
   float mx = -INFINITY, inv = 0.f;
+  float others = 0.f;  // softmax: what the largest score leaves of 1
   if (soft) {
 #pragma unroll
     for (int i = 0; i < PER; i += 4) {
@@ -520,50 +526,82 @@ __global__ void __launch_bounds__(256) route_groups_backward_kernel(const float*
       for (int z = 0; z < 4; ++z) l[i + z] = v[z], mx = fmaxf(mx, v[z]);
     }
     mx = max_lanes<W>(mx);
-    float sum = 0.f;
+    float most = 0.f, rest = 0.f;  // the terms at the maximum (each 1, or NaN), and below it
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
+      const bool at = l[i] == mx;
       l[i] = l[i] == -INFINITY ? 0.f : ex2((l[i] - mx) * kLog2e);  // from here on: the scores
-      sum += l[i];
+      most += at ? l[i] : 0.f;
+      rest += at ? 0.f : l[i];
     }
-    sum = sum_lanes<W>(sum);
+    most = sum_lanes<W>(most);
+    rest = sum_lanes<W>(rest);
+    const float sum = most + rest;
     inv = sum == 0.f ? 0.f : 1.f / sum;
+    others = (rest + (most - 1.f)) * inv;
   }
-  float total = 0.f;
+  float total = 0.f, left[SLOTS];  // left: 1 - s
 #pragma unroll
   for (int m = 0; m < SLOTS; ++m) {
     s[m] = e[m] < 0 || x[m] == -INFINITY ? 0.f : (soft ? expf(x[m] - mx) * inv : 1.f / (1.f + expf(-x[m])));
+    left[m] = !soft ? 1.f / (1.f + expf(x[m])) : (x[m] == mx ? others : 1.f - s[m]);  // (below the maximum: s <= 1/2)
     total += s[m];
   }
   float den, scale;
   bool follows;
   denominator(norm, k, route_scale, sum_lanes<W>(total), den, scale, follows);
-  float mean = 0.f;
-#pragma unroll
-  for (int m = 0; m < SLOTS; ++m)
-    if (e[m] >= 0) mean += g[m] * (s[m] / den);
-  mean = sum_lanes<W>(mean);  // (by the whole warp: the tokens of one may differ in `follows`)
-  if (!follows) mean = 0.f;
-  float mine[SLOTS], dot = 0.f;  // dL/ds * s of each slot
+  const float eps_den = follows && norm == MIRAI_NORM_EPS ? 1e-20f / den : 0.f;
+  float mean = 0.f, share[SLOTS];
 #pragma unroll
   for (int m = 0; m < SLOTS; ++m) {
-    mine[m] = e[m] >= 0 ? scale * ((g[m] - mean) / den) * s[m] : 0.f;
-    dot += mine[m];
+    share[m] = s[m] / den;
+    if (e[m] >= 0) mean += g[m] * share[m];
   }
-  dot = sum_lanes<W>(dot);
-  // slots that name the same expert share the sum of theirs
-  float sums[SLOTS];
+  mean = sum_lanes<W>(mean);
+  const float dot = scale * mean * (follows ? eps_den : 1.f);  // sum_j ds_j s_j
+  // Every pair of slots: a_j, and whether an expert is named twice.  (By the whole warp: the
+  // tokens of one may differ in `follows`.)
+  float a[SLOTS];
+  bool twice = false;
 #pragma unroll
-  for (int m = 0; m < SLOTS; ++m) sums[m] = 0.f;
+  for (int m = 0; m < SLOTS; ++m) a[m] = follows ? g[m] * eps_den : 0.f;
 #pragma unroll
   for (int m2 = 0; m2 < SLOTS; ++m2) {
     for (int j = 0; j < W && m2 * W + j < k; ++j) {
-      const int other = __shfl_sync(0xffffffffu, e[m2], (lane & ~(W - 1)) + j);
-      const float v = __shfl_sync(0xffffffffu, mine[m2], (lane & ~(W - 1)) + j);
+      const int from = (lane & ~(W - 1)) + j;
+      const int other = __shfl_sync(0xffffffffu, e[m2], from);
+      const float go = __shfl_sync(0xffffffffu, g[m2], from);
+      const float so = __shfl_sync(0xffffffffu, follows ? share[m2] : s[m2], from);
 #pragma unroll
-      for (int m = 0; m < SLOTS; ++m)
-        if (other == e[m]) sums[m] += v;
+      for (int m = 0; m < SLOTS; ++m) {
+        const bool same = other == e[m];
+        if (follows) {
+          a[m] = fmaf(g[m] - go, so, a[m]);
+          twice |= same && e[m] >= 0 && (m2 != m || j != li);
+        } else if (same) {  // (den fixed: a slot already holds its expert's sum)
+          a[m] = fmaf(go, soft ? left[m] : 1.f, a[m]);
+        } else if (soft) {
+          a[m] = fmaf(-go, so, a[m]);
+        }
+      }
     }
+  }
+  if (__any_sync(0xffffffffu, twice)) {  // slots that name the same expert share the sum of theirs
+    float sums[SLOTS];
+#pragma unroll
+    for (int m = 0; m < SLOTS; ++m) sums[m] = 0.f;
+#pragma unroll
+    for (int m2 = 0; m2 < SLOTS; ++m2) {
+      for (int j = 0; j < W && m2 * W + j < k; ++j) {
+        const int other = __shfl_sync(0xffffffffu, e[m2], (lane & ~(W - 1)) + j);
+        const float v = __shfl_sync(0xffffffffu, a[m2], (lane & ~(W - 1)) + j);
+#pragma unroll
+        for (int m = 0; m < SLOTS; ++m)
+          if (other == e[m]) sums[m] += v;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < SLOTS; ++m) a[m] = follows ? sums[m] : a[m];
   }
   const float tail = -inv * dot;
   if (live) {
@@ -586,7 +624,11 @@ __global__ void __launch_bounds__(256) route_groups_backward_kernel(const float*
   if (live) {
 #pragma unroll
     for (int m = 0; m < SLOTS; ++m)
-      if (e[m] >= 0) store_grad(grow + e[m], soft ? sums[m] - s[m] * dot : sums[m] * (1.f - s[m]));
+      if (e[m] >= 0) {
+        // den fixed, softmax: a is ds_e - sum_j ds_j s_j already (times den / scale)
+        const float d = scale * share[m] * a[m];
+        store_grad(grow + e[m], !soft ? d * left[m] : (follows ? d - s[m] * dot : d));
+      }
   }
 }
 
