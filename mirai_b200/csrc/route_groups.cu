@@ -232,7 +232,8 @@ __device__ __forceinline__ bool route_fast(const Args& a, int64_t t, bool write)
   }
   // Error of a score: ex2 and rcp are within 2^-22 of their values and the exponent's product
   // adds |x| 2^-24, times s (1 - s) <= 1/4 (and <= 0.23 / |x|), with two roundings of s: below
-  // 2^-21.9 for sigmoid; softmax as in route_row.
+  // 2^-21.9 for sigmoid.  A softmax's terms add the rounding of their arguments (2^-18.5 at 87, below which
+  // they are 0), their sum a few units more: below 2^-17 of the score, so of the largest.
   const float score_err = smax * (soft ? 0x1p-17f : 0x1.8p-22f);
   bool stays = group < a.G;
   if (a.top_groups < a.G) {
@@ -253,8 +254,13 @@ __device__ __forceinline__ bool route_fast(const Args& a, int64_t t, bool write)
       const uint32_t out = __ballot_sync(0xffffffffu, group < a.G && rank == a.top_groups) & team;
       const float worst_in = __shfl_sync(0xffffffffu, gv, __ffs(in) - 1);
       const float best_out = __shfl_sync(0xffffffffu, gv, __ffs(out) - 1);
-      if (best_out != kLow)
-        close |= worst_in - best_out <= 4.f * score_err + 0x1p-21f * (fabsf(worst_in) + fabsf(best_out) + smax);
+      // Every group has to keep clear of the middle by its own error: its scores', and the roundings of
+      // s + bias and of their sum, which are as large as the addends (a sum near 0 of large ones is not).
+      const bool two = a.top2 && best2 != kLow;
+      const float err = 2.f * score_err + 0x1p-22f * (fabsf(best1) + (two ? fabsf(best2) : 0.f) + smax);
+      const float mid = 0.5f * worst_in + 0.5f * best_out;
+      if (best_out != kLow && group < a.G && gv != kLow)
+        close |= !(rank < a.top_groups ? gv - mid > err : mid - gv > err);
     }
   }
   // leading bits of the key, then the id (lowest first), 0 for a closed slot

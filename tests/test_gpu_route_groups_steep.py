@@ -1,9 +1,10 @@
-"""Group-limited routing away from small logits: gradients of sure routers, whose scores leave little of 1."""
+"""Group-limited routing away from small logits and biases: gradients of sure routers, whose scores leave little of 1,
+and groups whose two best keys are far larger than their sum."""
 
 import pytest
 import torch
 
-from test_gpu_route_groups import _dev, grad64
+from test_gpu_route_groups import _dev, grad64, route64
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +120,33 @@ def test_gradient_of_saturated_and_repeated_experts():
             got = ops.route_groups_backward(gw.to(dev), inf.to(dev), idx.to(dev), score_func=score_func, norm=norm)
             assert torch.isfinite(got).all() and got[0, 5] == 0
     ops.check_device()
+
+
+@pytest.mark.parametrize("score_func", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("B", [4.0, 64.0, 4096.0])
+@pytest.mark.parametrize("large", ["all", "first"])
+def test_groups_of_two_large_keys_with_a_small_sum(score_func, B, large):
+    """Groups of two experts with biases near +B and -B: s + bias rounds at B 2^-24, the sums lie closer than that.  Groups
+    are chosen as in 64 bits, whether every group has such keys or only one that is not at the border."""
+    dev = _dev()
+    from mirai_b200 import ops
+    g = torch.Generator().manual_seed(int(B))
+    T, G, k = 400, 8, 2
+    base = torch.randn(T, 1, 2, generator=g)
+    near = base + (torch.rand(T, G, 2, generator=g) * 2 - 1) * 2.0 ** -22 * B  # sums apart by about their rounding
+    logits = near.reshape(T, 2 * G).float()
+    bias = torch.zeros(G, 2)
+    if large == "all":
+        bias[:, 0], bias[:, 1] = B, -B
+    else:
+        bias[0, 0], bias[0, 1] = B, -B
+    ids, _ = ops.route_groups(logits.to(dev), k, num_groups=G, top_groups=4, group_score="top2", score_func=score_func,
+                              choice_bias=bias.flatten().to(dev))
+    ops.check_device()
+    ref = route64(logits, k, G, 4, "top2", score_func, bias.flatten())
+    assert torch.equal(ids.cpu(), ref)
+    # the same with every member's logit closed but the first: its key alone counts
+    logits[:, 1::2] = -float("inf")
+    ids, _ = ops.route_groups(logits.to(dev), k, num_groups=G, top_groups=4, group_score="top2", score_func=score_func,
+                              choice_bias=bias.flatten().to(dev))
+    assert torch.equal(ids.cpu(), route64(logits, k, G, 4, "top2", score_func, bias.flatten()))
