@@ -150,3 +150,22 @@ def test_groups_of_two_large_keys_with_a_small_sum(score_func, B, large):
     ids, _ = ops.route_groups(logits.to(dev), k, num_groups=G, top_groups=4, group_score="top2", score_func=score_func,
                               choice_bias=bias.flatten().to(dev))
     assert torch.equal(ids.cpu(), route64(logits, k, G, 4, "top2", score_func, bias.flatten()))
+
+
+@pytest.mark.parametrize("E,G,top_groups,k", [(16, 1, 1, 4), (128, 8, 4, 8), (256, 16, 8, 8), (1000, 4, 3, 16), (1024, 1, 1, 10)])
+@pytest.mark.parametrize("score_func,group_score", [("sigmoid", "max"), ("softmax", "max"), ("sigmoid", "top2")])
+def test_ties_of_bf16_logits(E, G, top_groups, k, score_func, group_score):
+    """Logits on bf16's grid, most rows with equal ones at the cut: ids as in 64 bits, lowest first, from bf16, from the same
+    values in fp32, and from fp32 where one value of a row has low bits that the ids' would hide."""
+    dev = _dev()
+    from mirai_b200 import ops
+    g = torch.Generator().manual_seed(E)
+    lg = (torch.randn(60, E, generator=g) * 4).round().div(8 if E < 100 else 16).bfloat16()
+    lg[::7, ::3] = -float("inf")
+    odd = lg.float()
+    odd[torch.arange(60), torch.randint(E, (60,), generator=g)] += 2.0 ** -21
+    how = {"num_groups": G, "top_groups": top_groups, "group_score": group_score, "score_func": score_func}
+    for x in (lg, lg.float(), odd):
+        ids, _ = ops.route_groups(x.to(dev), k, **how)
+        ops.check_device()
+        assert torch.equal(ids.cpu(), route64(x.float(), k, G, top_groups, group_score, score_func, None))
