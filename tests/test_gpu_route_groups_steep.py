@@ -169,3 +169,24 @@ def test_ties_of_bf16_logits(E, G, top_groups, k, score_func, group_score):
         ids, _ = ops.route_groups(x.to(dev), k, **how)
         ops.check_device()
         assert torch.equal(ids.cpu(), route64(x.float(), k, G, top_groups, group_score, score_func, None))
+
+
+@pytest.mark.parametrize("k,top_groups", [(2, 1), (3, 2), (6, 3)])
+def test_block_tokens_use_their_best_groups(k, top_groups):
+    """The groups of a token's experts, counted token by token, and which they are, against 64 bits."""
+    dev = _dev()
+    from mirai_b200 import block
+    T, H, E, G = 100, 64, 16, 4
+    g = torch.Generator().manual_seed(k)
+    # (values on a grid: the logits are the same in fp32 and in 64 bits)
+    x = torch.randint(-8, 9, (T, H), generator=g) / 8
+    weight = torch.randint(-8, 9, (E, H), generator=g) / 64
+    bias = torch.randn(E, generator=g) * 0.05
+    idx, _ = block.route(x.to(dev), weight.to(dev), top_k=k, correction_bias=bias.to(dev), num_groups=G,
+                         top_groups=top_groups)
+    idx = idx.cpu()
+    assert torch.equal(idx, route64(x.double() @ weight.double().T, k, G, top_groups, "top2", "sigmoid", bias))
+    used = [len(set((row // (E // G)).tolist())) for row in idx]
+    assert max(used) <= top_groups
+    free, _ = block.route(x.to(dev), weight.to(dev), top_k=k, correction_bias=bias.to(dev))
+    assert max(len(set((row // (E // G)).tolist())) for row in free.cpu()) > top_groups  # the limit is what keeps them
