@@ -478,6 +478,18 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// An odd number of blocks (K % 64 == 32): the last K = 64 step reads one block past the row, whose codes
+// are zeros (TMA fill).  Its scale must not be the NaN byte, which a key's padding may hold: the words' byte
+// is cleared.  `blocks`: those of the last k-block; four per word, two words (K tiles) per row.
+struct PadMask {
+  uint32_t keep0, keep1;
+};
+__device__ __forceinline__ PadMask pad_mask(int blocks) {
+  const uint32_t m = ~(0xffu << (8 * (blocks & 3)));
+  return PadMask{blocks < 4 ? m : ~0u, blocks < 4 ? ~0u : m};
+}
+__device__ __forceinline__ void keep_bytes(uint4& v, uint32_t m) { v.x &= m, v.y &= m, v.z &= m, v.w &= m; }
+
 // Bring a box of a tensor map into L2.
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
@@ -874,8 +886,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_after();  // the MMAs that read this slot have completed (the stage was refilled after them)
           const uint32_t src = smem_u32(sSF + rb.i * SF_BYTES) + lane * 16u;
           const uint32_t dst = tmem + SF_COL + rb.i * 32 + quarter;
-          const uint4 a0 = lds128(src), a1 = lds128(src + 512);
-          const uint4 l0 = lds128(src + 1024), l1 = lds128(src + 1536), h0 = lds128(src + 2048), h1 = lds128(src + 2560);
+          uint4 a0 = lds128(src), a1 = lds128(src + 512);
+          uint4 l0 = lds128(src + 1024), l1 = lds128(src + 1536), h0 = lds128(src + 2048), h1 = lds128(src + 2560);
+          if (kb == num_kb - 1 && p.K % 64) {
+            const PadMask m = pad_mask(p.K % BKE / 32);
+            keep_bytes(a0, m.keep0), keep_bytes(l0, m.keep0), keep_bytes(h0, m.keep0);
+            keep_bytes(a1, m.keep1), keep_bytes(l1, m.keep1), keep_bytes(h1, m.keep1);
+          }
           tmem_st_x8(dst, a0, a1);
           tmem_st_x8(dst + 8, l0, h0);    // K tile 0: both column halves
           tmem_st_x8(dst + 16, l1, h1);   // K tile 1
@@ -1317,8 +1334,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         tc_fence_after();
         const uint32_t src = smem_u32(sSF + r.i * KEYS * 1024) + lane * 16u;
         const uint32_t dst = tmem + FEW_SF_COL + r.i * 32 + quarter;
-        tmem_st_x8(dst, lds128(src), lds128(src + 512));
-        if (KEYS == 2) tmem_st_x8(dst + 8, lds128(src + 1024), lds128(src + 1536));
+        const bool pad = kb == num_kb - 1 && p.K % 64;
+        const PadMask pm = pad_mask(p.K % BKE / 32);
+#pragma unroll
+        for (int key = 0; key < KEYS; ++key) {
+          uint4 w0 = lds128(src + key * 1024), w1 = lds128(src + key * 1024 + 512);
+          if (pad) keep_bytes(w0, pm.keep0), keep_bytes(w1, pm.keep1);
+          tmem_st_x8(dst + 8 * key, w0, w1);
+        }
         tmem_st_x8(dst + 16, make_uint4(sXS[2 * kb * 32 + lane], 0, 0, 0), make_uint4(sXS[(2 * kb + 1) * 32 + lane], 0, 0, 0));
         tmem_st_wait();
         tc_fence_before();
