@@ -107,6 +107,10 @@ class CudaStepOps:
         (NF4 keys decoded once to bf16 where that pays: ``ops.stage_nf4``)."""
         return self.ops.stage_nf4(tuple(weights), rows, weights[0].shape[0], training=training)
 
+    def check_train(self, weights, hidden, inter):
+        """Refuse a training pass that its backward could not run (before any exchange)."""
+        self.ops.check_mxfp4_training(weights, hidden, inter)
+
     def experts_train(self, x_sorted, offsets, weights, inter, sources=1, save=True, lora=None):
         """The owner's GEMMs over its received (source, expert) segments; the
         block-Hadamard INT8 format rotates the received rows and h here (a row's
@@ -114,6 +118,8 @@ class CudaStepOps:
         rank's experts' factors) runs on the same segments: its projections and
         rank blocks read each segment's expert."""
         w1, w3, w2 = weights
+        if save:
+            self.check_train(weights, x_sorted.shape[1], inter)
         g_in, g_mid = self.ops._rotations(w1, w3, w2)
         x = self.ops.rotate_rows(x_sorted, g_in) if g_in else x_sorted
         res = self.ops.gateup_swiglu(x, offsets, w1, w3, inter=inter, sources=sources, save_gate_up=save)
@@ -196,6 +202,12 @@ def _weights_for(staged, local_weights):
     return local_weights
 
 
+def _check_train(ops, weights, hidden: int, inter: int) -> None:
+    f = getattr(ops, "check_train", None)
+    if f is not None:
+        f(weights, hidden, inter)
+
+
 def ep_moe_forward(tokens: torch.Tensor, logits: torch.Tensor, local_weights: Any, *, shard: ExpertShard,
                    top_k: int, inter: int, group=None, ops: StepOps | None = None, chunks: int = 1,
                    comm_stream: torch.cuda.Stream | None = None, train: bool = False, lora=None):
@@ -226,6 +238,8 @@ def ep_moe_forward(tokens: torch.Tensor, logits: torch.Tensor, local_weights: An
     G, E, El = shard.world, shard.num_experts, shard.local
     T, H = tokens.shape
     dev = tokens.device
+    if train:
+        _check_train(ops, local_weights, H, inter)
     if G == 1:  # one rank owns every expert: no exchange
         idx, tw = ops.route(logits, top_k)
         plan = ops.plan(idx, E)
@@ -785,6 +799,8 @@ class ExpertParallelMoE:
         if G == 1:
             return ep_moe_forward(tokens, logits, local_weights, shard=shard, top_k=k, inter=self.inter, ops=ops,
                                   train=train, lora=lora)
+        if train:
+            _check_train(ops, local_weights, H, self.inter)
         self._gen += 1
         if self.comm is None:
             self.comm = torch.cuda.Stream(device=dev)

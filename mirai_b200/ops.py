@@ -1305,14 +1305,18 @@ def _read_back_beside(weights):
     return outs, (lambda n: main.wait_event(events[n - 1]))
 
 
+def check_mxfp4_training(weights, hidden: int, inter: int) -> None:
+    """ValueError for MXFP4 keys of widths that the dX GEMMs do not take."""
+    if any(isinstance(w, Mxfp4Tensor) for w in weights) and (hidden % 64 or inter % 64):
+        raise ValueError(f"training MXFP4 experts needs hidden and inter in steps of 64, got {hidden} and {inter}")
+
+
 def moe_forward_train(tokens, top_indices, top_weights, w1, w3, w2, *, num_experts: int, inter: int,
                       out_dtype: torch.dtype | None = None, lora: DownLoRA | None = None):
     """Forward that also returns the state the dX pass consumes.  (MXFP4 keys:
     the forward takes widths in steps of 32, the backward of 64.)"""
     if any(isinstance(w, Mxfp4Tensor) for w in (w1, w3, w2)):
-        if tokens.shape[1] % 64 or inter % 64:
-            raise ValueError(f"training MXFP4 experts needs hidden and inter in steps of 64, got {tokens.shape[1]} and "
-                             f"{inter}")
+        check_mxfp4_training((w1, w3, w2), tokens.shape[1], inter)
         plan = dispatch_plan(top_indices, num_experts)
         y, gu, h, low = _mxfp4_experts(tokens, plan, w1, w3, w2, inter=inter, lora=lora, train=True)
         out = combine(y, plan.inverse_order, top_weights, out_dtype=out_dtype or tokens.dtype)
