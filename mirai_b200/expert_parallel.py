@@ -130,6 +130,10 @@ class CudaStepOps:
         keep = lora is not None and lora.compute_grads
         return y, (gu, h if keep else None, low if keep else None)
 
+    def read_back(self, weights):
+        """The weights a layer's backward multiplies: MXFP4 keys decoded once for all its chunks."""
+        return self.ops.mxfp4_read_back(weights)
+
     def experts_backward(self, grad_y, offsets, weights, inter, sources, saved, lora=None):
         if isinstance(saved, tuple) and saved and isinstance(saved[0], str):
             _, order, inverse, ends, inner = saved
@@ -200,6 +204,13 @@ def _weights_for(staged, local_weights):
     if staged is not None and all(a is b for a, b in zip(staged[0], local_weights)):
         return staged[1]
     return local_weights
+
+
+def _read_back(ops, weights, rows: int):
+    """The weights a backward over ``rows`` received rows multiplies in all its chunks
+    (``CudaStepOps.read_back``)."""
+    f = getattr(ops, "read_back", None)
+    return weights if f is None or rows == 0 else f(weights)
 
 
 def _check_train(ops, weights, hidden: int, inter: int) -> None:
@@ -387,7 +398,9 @@ def ep_moe_backward(grad_out: torch.Tensor, state: EPTrainState, local_weights: 
     gate/up dX run over the same source-major segments; dX rows travel back
     and the token owner sums each token's routes (the permute backward,
     dispatch_ops.py:15-20).  Every row's products are those of the single-GPU
-    backward, so the result equals it."""
+    backward, so the result equals it (MXFP4 keys: within the rounding of the rows
+    that travel, which are bf16 and weighted; the single-GPU layer keeps them in
+    fp32).  MXFP4 keys are read back once, for all the chunks."""
     ops = ops or CudaStepOps()
     G = shard.world
     k, H = state.top_k, state.hidden
@@ -398,7 +411,8 @@ def ep_moe_backward(grad_out: torch.Tensor, state: EPTrainState, local_weights: 
     dev = grad_out.device
     dx = torch.empty((T, H), dtype=state.dtype, device=dev)
     dw = torch.empty((T, k), dtype=torch.float32, device=dev)
-    local_weights = _weights_for(state.staged, local_weights)
+    rows = T * k if G == 1 else sum(sum(st["rc"]) for st in state.chunks)
+    local_weights = _read_back(ops, _weights_for(state.staged, local_weights), rows)
     state.staged = None
     for (b, e), st in zip(state.bounds, state.chunks):
         plan = st["plan"]
@@ -944,7 +958,7 @@ class ExpertParallelMoE:
         ex = _Exchange(self, state.ptrs, comp)
         dx = torch.empty((T, H), dtype=state.dtype, device=dev)
         dw = torch.empty((T, k), dtype=torch.float32, device=dev)
-        local_weights = _weights_for(state.staged, local_weights)
+        local_weights = _read_back(ops, _weights_for(state.staged, local_weights), sum(plan.in_rows))
         state.staged = None
         sent = []
         for c, (b, e) in enumerate(state.bounds):

@@ -635,9 +635,26 @@ def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: 
     return y
 
 
+class Mxfp4ReadBack:
+    """An MXFP4 key with its values read back to bf16 (``mxfp4_read_back``): ``down_dx`` and
+    ``gateup_dx`` take it for the key, and several calls on it decode it once."""
+
+    def __init__(self, key: Mxfp4Tensor):
+        self.key, self.shape, self.device = key, key.shape, key.device
+        self.dense = mxfp4_dequantize(key)
+
+
+def mxfp4_read_back(weights) -> tuple:
+    """``weights`` for a backward pass of several calls: MXFP4 keys as ``Mxfp4ReadBack`` (2 bytes per
+    weight while they are kept), others as given."""
+    return tuple(Mxfp4ReadBack(w) if isinstance(w, Mxfp4Tensor) else w for w in weights)
+
+
 def _dx_weight(w):
     """The weight a dX product multiplies: an MXFP4 key is read back (the scales run
     along the other axis than dX reduces over), others as given."""
+    if isinstance(w, Mxfp4ReadBack):
+        return w.dense
     return mxfp4_dequantize(w) if isinstance(w, Mxfp4Tensor) else w
 
 
@@ -931,6 +948,9 @@ def down_dx(grad_y: torch.Tensor, offsets: torch.Tensor, w2, gate_up: torch.Tens
     if isinstance(w2, Mxfp4Tensor):
         return _down_dx_mxfp4(grad_y, offsets, w2, gate_up, inter=inter, out=out, lora=lora, rank_a=rank_a,
                               sources=sources)
+    if isinstance(w2, Mxfp4ReadBack):
+        return _down_dx_mxfp4(grad_y, offsets, w2.key, gate_up, inter=inter, out=out, lora=lora, rank_a=rank_a,
+                              sources=sources, dense=w2.dense)
     group = getattr(w2, "group_size", 0)  # block-Hadamard INT8: the rotation group of dh
     w2 = _as_weight(w2)
     gy = _cuda(grad_y, "grad_y", torch.bfloat16)
