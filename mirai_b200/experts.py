@@ -405,6 +405,9 @@ class B200GroupedExperts(nn.Module):
                                          nested_absmax=buf["nf4_nabsmax"], offset=buf["nf4_offset"],
                                          code=buf["nf4_code"], nested_code=buf["nf4_ncode"], shape=shape, meta=meta)
             elif fmt == "mxfp4":
+                codes = tuple(buf["mxfp4"].shape)
+                if codes != (*shape[:-1], shape[-1] // 2) or shape[-1] % 2:
+                    raise ValueError(f"packed {key}_mxfp4: codes of shape {codes} for the entry's shape {shape}")
                 m.load_mxfp4_weight(key, packed=buf["mxfp4"], scale=buf["mxfp4_scale"])
             else:
                 m.load_quantized_weight(key, weight_int8=buf["int8"], weight_scale=buf["scale"],

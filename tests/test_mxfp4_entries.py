@@ -1,0 +1,26 @@
+"""MXFP4 buffers as a layer is given them (no GPU): entries that contradict themselves, tensors that start off their place."""
+
+import pytest
+import torch
+
+from mirai_b200 import experts as ex
+
+
+def entry(E, H, I, shape_of):
+    names, tensors, shapes = {}, {}, {}
+    for key, (o, i) in {"w1": (I, H), "w3": (I, H), "w2": (H, I)}.items():
+        names[f"{key}_mxfp4"], names[f"{key}_mxfp4_scale"] = f"ffn.{key}", f"ffn.{key}.scale"
+        tensors[f"ffn.{key}"] = torch.zeros(E, o, i // 2, dtype=torch.uint8)
+        tensors[f"ffn.{key}.scale"] = torch.full((E, o, i // 32), 127, dtype=torch.uint8)
+        shapes[key] = shape_of(key, [E, o, i])
+    return {"kind": "grouped_experts", "quant_format": "mxfp4", "num_experts": E, "tensors": names, "shapes": shapes}, tensors
+
+
+@pytest.mark.parametrize("wrong", [lambda s: [s[0], s[1], s[2] + 32], lambda s: [s[0], s[2], s[1]], lambda s: s[1:],
+                                   lambda s: [s[0], s[1], s[2] + 1]])
+@pytest.mark.parametrize("at", ["w1", "w2"])
+def test_a_packed_entry_whose_shapes_are_not_its_codes(wrong, at):
+    good = ex.B200GroupedExperts.from_packed_state(*entry(2, 64, 96, lambda k, s: s))
+    assert good.is_fully_loaded()
+    with pytest.raises(ValueError, match=f"{at}_mxfp4: codes of shape"):
+        ex.B200GroupedExperts.from_packed_state(*entry(2, 64, 96, lambda k, s: wrong(s) if k == at else s))
