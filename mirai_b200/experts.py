@@ -545,7 +545,9 @@ class B200GroupedExperts(nn.Module):
         if not problems and tuple(scale.shape) != tiles:
             problems.append(f"{key}_mxfp4_scale: shape {tuple(scale.shape)}, expected {tiles}")
         _require(problems, f"MXFP4 buffers for {key}")
-        self._install(key, "mxfp4", {"mxfp4": packed.detach().contiguous(), "mxfp4_scale": scale.detach().contiguous()})
+        # (aligned here: a copy made at binding would miss what is later written into the buffers)
+        self._install(key, "mxfp4", {"mxfp4": ops._aligned(packed.detach().contiguous()),
+                                     "mxfp4_scale": ops._aligned(scale.detach().contiguous())})
 
     def is_fully_loaded(self) -> bool:
         return self._loaded.issuperset({"w1", "w2", "w3"})

@@ -24,3 +24,18 @@ def test_a_packed_entry_whose_shapes_are_not_its_codes(wrong, at):
     assert good.is_fully_loaded()
     with pytest.raises(ValueError, match=f"{at}_mxfp4: codes of shape"):
         ex.B200GroupedExperts.from_packed_state(*entry(2, 64, 96, lambda k, s: wrong(s) if k == at else s))
+
+
+def test_buffers_that_start_off_alignment_are_installed_aligned():
+    """Views into a file's bytes can start anywhere. What the kernels read has to be the module's buffer itself, so that a state
+    loaded into it later is seen."""
+    E, o, i = 2, 96, 64
+    codes = torch.arange(E * o * i // 2 + 5, dtype=torch.int32).to(torch.uint8)[5:].view(E, o, i // 2)
+    tiles = torch.arange(E * 512 + 3, dtype=torch.int32).to(torch.uint8)[3:].view(E, 1, 1, 512)
+    m = ex.B200GroupedExperts.from_empty(num_experts=E, quant_format="mxfp4")
+    m.load_mxfp4_weight("w1", packed=codes, scale=tiles)
+    for buf, given in ((m.w1_mxfp4, codes), (m.w1_mxfp4_scale, tiles)):
+        assert given.data_ptr() % 32 and buf.data_ptr() % 32 == 0 and torch.equal(buf, given)
+    aligned = codes.clone()
+    m.load_mxfp4_weight("w3", packed=aligned, scale=tiles.clone())
+    assert m.w3_mxfp4.data_ptr() == aligned.data_ptr()  # used in place
