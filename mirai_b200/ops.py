@@ -600,6 +600,11 @@ def _gateup_mxfp4(x, offsets: torch.Tensor, w1: Mxfp4Tensor, w3: Mxfp4Tensor, *,
     return h, gu, hq
 
 
+def _check_rank_rows(low: torch.Tensor, rows: int) -> None:
+    if tuple(low.shape) != (rows, 64) or low.dtype != torch.bfloat16 or not low.is_contiguous():
+        raise ValueError(f"rank_a must be contiguous bf16 [{rows}, 64], got {low.dtype} {tuple(low.shape)}")
+
+
 def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: torch.Tensor | None,
                 lora: "DownLoRA | None", rank_a: torch.Tensor | None, sources: int) -> torch.Tensor:
     E, out_f, inter = w2.shape
@@ -620,8 +625,7 @@ def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: 
         if rank_a is None and isinstance(h, Mxfp4Rows):
             raise ValueError("a LoRA adapter on quantised rows needs rank_a, its projection of the bf16 rows")
         low = rank_a if rank_a is not None else lora_project(h, offsets, lora, forward=True, sources=sources)
-        if tuple(low.shape) != (h.shape[0], 64) or low.dtype != torch.bfloat16 or not low.is_contiguous():
-            raise ValueError(f"rank_a must be contiguous bf16 [{h.shape[0]}, 64], got {low.dtype} {tuple(low.shape)}")
+        _check_rank_rows(low, h.shape[0])
         rank_b = lora.b_pad()
         if rank_b.shape[0] != E * hidden:
             raise ValueError(f"the adapter's B has {rank_b.shape[0]} rows, the key {E} x {hidden}")
@@ -1006,7 +1010,11 @@ def _down_dx_mxfp4(grad_y, offsets, w2: Mxfp4Tensor, gate_up, *, inter: int, out
     low = rank_b = None
     if lora is not None:
         low = rank_a if rank_a is not None else lora_project(gy, offsets, lora, forward=False, sources=sources)
+        _check_rank_rows(low, S)
         rank_b = lora.a_pad()
+        if rank_b.numel() != E * 64 * inter:
+            raise ValueError(f"the adapter's A has {rank_b.numel()} padded entries, the key needs {E} x 64 x {inter}")
+        _same_device(w2.device, lora=rank_b)
     dgu = _mxfp4_output(out, (S, 2 * inter), w2.device)
     if wide:
         _run(w2.device, "mirai_moe_down_dx_rows_f32", gy.data_ptr(), _ptr(row_weights), offsets.data_ptr(), sources, E, S,

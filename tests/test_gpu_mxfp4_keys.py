@@ -30,3 +30,24 @@ def test_padding_scales_of_a_key_do_not_count(K, N, few, monkeypatch):
         ops.check_device()
         assert torch.isfinite(got.float()).all() and torch.equal(got, want)
     assert torch.equal(ops.mxfp4_dequantize(dirty[0]), ops.mxfp4_dequantize(clean[0]))
+
+
+def test_down_dx_refuses_an_adapter_that_does_not_fit():
+    """The rank block's operands are read by the rows and channels of the call: others are refused before the product."""
+    dev = _dev()
+    from mirai_b200 import ops
+    E, H, I, counts = 2, 64, 128, [5, 9]
+    S, off = sum(counts), segments(counts, dev)
+    w2 = ops.mxfp4_quantize(weight(E, H, I, dev))
+    gy, lora = rows(S, H, dev), ops.DownLoRA(weight(E, 4, I, dev), weight(E, H, 4, dev), 1.0)
+    low = torch.zeros(S, 64, dtype=torch.bfloat16, device=dev)
+    for dtype in (torch.bfloat16, torch.float32):
+        gu = torch.randn(S, 2 * I, device=dev).to(dtype)
+        ops.down_dx(gy, off, w2, gu, inter=I, lora=lora, rank_a=low)
+        for bad in (low[1:], low[:, :32], low.float(), low.repeat(1, 2)[:, ::2]):
+            with pytest.raises(ValueError, match="rank_a must be"):
+                ops.down_dx(gy, off, w2, gu, inter=I, lora=lora, rank_a=bad)
+        other = ops.DownLoRA(weight(E, 4, I // 2, dev), weight(E, H, 4, dev), 1.0)
+        with pytest.raises(ValueError, match="adapter's A"):
+            ops.down_dx(gy, off, w2, gu, inter=I, lora=other, rank_a=low)
+    ops.check_device()
