@@ -532,11 +532,18 @@ def _mxfp4_rows(x, offsets: torch.Tensor, width: int, name: str) -> Mxfp4Rows:
 
 
 # bf16 rows are quantised inside the product (few_rows_kernel in mxfp4.cu) up to this many, and up to 16
-# rows per segment: measured (H 2048, I 1408, 32 experts; quantise + product against it, gate/up and down, us)
-# 16 rows 29.7 / 25.6 against 17.3 / 17.3, 512 rows 48.1 / 35.8 against 38.9 / 32.8, 1024 rows 52.2 / 39.9
-# against 54.1 / 47.1.
+# rows per segment (1024 at most).  Measured, gate/up, us, quantise + product against it (cold L2):
+#   H 2048, I 1408    1 expert: 256 rows 27.6 / 19.4, 512 rows 27.6 / 28.7;  8: 256 rows 31.7 / 20.5, 1024 rows 33.8 / 41.0
+#                     32: 512 rows 48.1 / 41.0, 1024 rows 52.2 / 49.2;     128: 256 rows 103 / 87, 1024 rows 106 / 90
+#   H 4096, I 1536    1: 256 rows 37.9 / 26.6, 512 rows 37.9 / 45.1;       32: 512 rows 74.7 / 68.6;  128: 1024 rows 181 / 170
+#   H 1024, I 512     every case up to 1024 rows is faster in one launch (1 expert: 1024 rows 21.5 / 16.4)
+# down has half the weights per tile in flight, so that many experts stream better through the general
+# product: it takes up to MXFP4_FEW_ROWS rows on up to 64 segments that can have rows.
+#   H 2048, I 1408    1: 256 rows 25.6 / 16.4;  32: 256 rows 29.7 / 26.6, 512 rows 31.7 / 32.8;  128: 64 rows 44.0 / 41.0, 128 rows 62.5 / 69.6
+#   H 4096, I 1536    1: 256 rows 25.6 / 22.5;  32: 256 rows 42.0 / 43.0;  128: 32 rows 42.0 / 41.0, 64 rows 64.5 / 69.6, 128 rows 99 / 123
 MXFP4_FEW_ROWS = 256
 MXFP4_FEW_ROWS_PER_SEGMENT = 16
+MXFP4_FEW_DOWN_SEGMENTS = 64
 _FEW_MAX_ROWS, _FEW_MAX_WIDTH = 1024, 4096
 
 
@@ -546,6 +553,11 @@ def _few_limit(segments: int) -> int:
 
 def _few_rows(x, width: int, segments: int) -> bool:
     return isinstance(x, torch.Tensor) and width <= _FEW_MAX_WIDTH and x.shape[0] <= _few_limit(segments)
+
+
+def _few_rows_down(x, width: int, segments: int) -> bool:
+    return (_few_rows(x, width, segments) and x.shape[0] <= MXFP4_FEW_ROWS
+            and min(x.shape[0], segments) <= MXFP4_FEW_DOWN_SEGMENTS)
 
 
 def _few_input(x: torch.Tensor, width: int, name: str) -> torch.Tensor:
@@ -614,7 +626,7 @@ def _down_mxfp4(h, offsets: torch.Tensor, w2: Mxfp4Tensor, *, hidden: int, out: 
                          f"segments of {sources} source(s)")
     device = w2.device
     _same_device(device, h=h, offsets=offsets, rank_a=rank_a)
-    if lora is None and _few_rows(h, inter, offsets.numel()):
+    if lora is None and _few_rows_down(h, inter, offsets.numel()):
         h = _few_input(h, inter, "h")
         y = _mxfp4_output(out, (h.shape[0], hidden), device)
         _run(device, "mirai_moe_down_mxfp4_few", h.data_ptr(), offsets.data_ptr(), sources, E, h.shape[0], inter, hidden,

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from mirai_b200 import experts as ex
+from mirai_b200 import ops
 
 
 def entry(E, H, I, shape_of):
@@ -39,3 +40,14 @@ def test_buffers_that_start_off_alignment_are_installed_aligned():
     aligned = codes.clone()
     m.load_mxfp4_weight("w3", packed=aligned, scale=tiles.clone())
     assert m.w3_mxfp4.data_ptr() == aligned.data_ptr()  # used in place
+
+
+def test_which_rows_are_quantised_inside_the_product():
+    """Up to 256 rows or 16 a segment for gate/up, 1024 at most; down up to 256 rows on up to 64 segments that can have rows."""
+    def of(rows, segments, width=2048):
+        x = torch.empty(rows, width, dtype=torch.bfloat16, device="meta")
+        return ops._few_rows(x, width, segments), ops._few_rows_down(x, width, segments)
+
+    assert of(1, 1) == of(256, 8) == of(256, 64) == of(64, 128) == (True, True)
+    assert of(257, 8) == of(1025, 1024) == of(16, 8, 4128) == (False, False)
+    assert of(512, 32) == of(65, 128) == of(200, 128) == of(1024, 64) == (True, False)
