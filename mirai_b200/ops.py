@@ -894,8 +894,10 @@ def combine(y_sorted: torch.Tensor, inverse_order: torch.Tensor, top_weights: to
         if out.dtype != torch.bfloat16:
             raise TypeError("bf16 accumulation writes a bf16 output")
         code = COMBINE_BF16_ACCUM
-    _lib.call("mirai_moe_combine_f32" if rows_f32 else "mirai_moe_combine", _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H,
-              _ptr(out), code, _stream())
+    if rows_f32:
+        _run(y_sorted.device, "mirai_moe_combine_f32", _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H, _ptr(out), code)
+        return out
+    _lib.call("mirai_moe_combine", _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H, _ptr(out), code, _stream())
     return out
 
 
@@ -932,8 +934,9 @@ def combine_backward_rows(grad_out: torch.Tensor, y_sorted: torch.Tensor, invers
     rows = torch.empty_like(y_sorted)
     rw = torch.empty(T * k, dtype=torch.float32, device=g.device)
     gw = torch.empty((T, k), dtype=torch.float32, device=g.device)
-    _lib.call("mirai_moe_combine_backward_rows", _ptr(g), _ptr(y_sorted), _ptr(inv), _ptr(w), T, k, H, _ptr(rows),
-              _ptr(rw), _ptr(gw), _stream())
+    _same_device(g.device, y_sorted=y_sorted, inverse_order=inv, top_weights=w)
+    _run(g.device, "mirai_moe_combine_backward_rows", g.data_ptr(), y_sorted.data_ptr(), inv.data_ptr(), w.data_ptr(), T, k,
+         H, rows.data_ptr(), rw.data_ptr(), gw.data_ptr())
     return rows, rw, gw
 
 

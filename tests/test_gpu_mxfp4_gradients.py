@@ -242,3 +242,27 @@ def test_dx_beside_an_adapter():
         dx.index_add_(0, t, (dh * u * sg * (1 + gt * (1 - sg))) @ w1[e] + (dh * gt * sg) @ w3[e])
     assert norm_error(x.grad, dx) <= 1.85 * norm_error(dx.bfloat16(), dx)
     assert norm_error(ad.lora_a.grad, dA) < 0.008 and norm_error(ad.lora_b.grad, dB) < 0.008
+
+
+@pytest.mark.parametrize("T", [0, 1])
+def test_layer_of_no_token_and_of_one(T):
+    """Nothing to compute, and a token whose second weight is 0: its route adds nothing to dx."""
+    dev = _dev()
+    from mirai_b200 import experts as ex
+    from mirai_b200 import ops
+    E, H, I = 3, 64, 128
+    m = ex.B200GroupedExperts.from_empty(num_experts=E, quant_format="mxfp4")
+    for i, (key, shape) in enumerate({"w1": (I, H), "w3": (I, H), "w2": (H, I)}.items()):
+        m.load_dense_weight(key, weight(E, *shape, dev, i + 1))
+    x = rows(T, H, dev).requires_grad_()
+    idx = torch.tensor([[2, 0]] * T, dtype=torch.int64, device=dev).view(T, 2)
+    score = torch.tensor([[0.75, 0.0]] * T, device=dev).view(T, 2).requires_grad_()
+    grad = torch.ones(T, H, dtype=torch.bfloat16, device=dev)
+    out = m.run_direct_routed(x, score, idx)
+    dx, ds = torch.autograd.grad(out, [x, score], grad)
+    ops.check_device()
+    assert out.shape == dx.shape == (T, H) and ds.shape == (T, 2)
+    if T:
+        one = x.detach().requires_grad_()
+        same = m.run_direct_routed(one, score[:, :1].detach(), idx[:, :1].contiguous())
+        assert torch.equal(torch.autograd.grad(same, one, grad)[0], dx) and (ds != 0).all()
