@@ -1598,6 +1598,8 @@ static int few_product(const char* name, const void* x, const int32_t* offsets, 
   if (gate_up_dtype != MIRAI_DTYPE_BF16 && gate_up_dtype != MIRAI_DTYPE_F32)
     return set_error(MIRAI_ERR_INVALID_ARG, "%s: gate/up is saved in bf16 or fp32 (dtype %d)", name, gate_up_dtype);
   if (misaligned(x, 32)) return set_error(MIRAI_ERR_INVALID_ARG, "%s: rows not 32-byte aligned", name);
+  if (misaligned(out, 2) || misaligned(gate_up, gate_up_dtype == MIRAI_DTYPE_F32 ? 4 : 2))
+    return set_error(MIRAI_ERR_INVALID_ARG, "%s: output not aligned to its type", name);
   const int kt = (int)ceil_div(K, 128);
   FewParams p = {};
   p.x = static_cast<const __nv_bfloat16*>(x);

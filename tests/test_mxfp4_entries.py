@@ -3,8 +3,10 @@
 import pytest
 import torch
 
+from mirai_b200 import _lib, ops
 from mirai_b200 import experts as ex
-from mirai_b200 import ops
+
+ALIGNED = 4096  # an address for checks that end before any launch
 
 
 def entry(E, H, I, shape_of):
@@ -51,3 +53,42 @@ def test_which_rows_are_quantised_inside_the_product():
     assert of(1, 1) == of(256, 8) == of(256, 64) == of(64, 128) == (True, True)
     assert of(257, 8) == of(1025, 1024) == of(16, 8, 4128) == (False, False)
     assert of(512, 32) == of(65, 128) == of(200, 128) == of(1024, 64) == (True, False)
+
+
+def test_c_entries_refuse_types_and_addresses():
+    """What the C entries see before any launch."""
+    from mirai_b200.build import build
+    build()
+    lib = _lib.load()
+
+    def refused(code, text, name, *args):
+        assert getattr(lib, name)(*args) == code and text in lib.mirai_b200_last_error()
+
+    A, w = ALIGNED, _lib.Mxfp4Weight(ALIGNED, ALIGNED)
+    few, save = "mirai_moe_gateup_swiglu_mxfp4_few_save", "mirai_moe_gateup_swiglu_mxfp4_save"
+    refused(1, b"bf16 or fp32", few, A, A, 1, 1, 8, 64, 64, w, w, A, A, 3, None)
+    refused(1, b"aligned to its type", few, A, A, 1, 1, 8, 64, 64, w, w, A + 1, A, 0, None)
+    refused(1, b"aligned to its type", few, A, A, 1, 1, 8, 64, 64, w, w, A, A + 2, 1, None)
+    refused(1, b"aligned to its type", "mirai_moe_gateup_swiglu_mxfp4_few", A, A, 1, 1, 8, 64, 64, w, w, A, A + 1, None)
+    refused(1, b"aligned to its type", "mirai_moe_down_mxfp4_few", A, A, 1, 1, 8, 64, 64, w, A + 1, None)
+    refused(1, b"bf16 or fp32", save, A, A, A, 1, 1, 8, 64, 64, w, w, A, A, 3, None, None, None)
+    refused(1, b"16-byte", save, A, A, A, 1, 1, 8, 64, 64, w, w, A, A + 8, 1, None, None, None)
+    rows, dx = "mirai_moe_down_dx_rows_f32", "mirai_moe_gateup_dx_f32"
+    refused(1, b"null rank-block", rows, A, A, A, 1, 1, 8, 64, 64, A, A, A, None, A, None)
+    refused(1, b"segments", rows, A, A, A, 2, 513, 8, 64, 64, A, A, None, None, A, None)
+    refused(1, b"saved gate/up", rows, A, None, A, 1, 1, 8, 64, 64, A, None, None, None, A, None)
+    refused(2, b"% 64", rows, A, None, A, 1, 1, 8, 96, 64, A, A, None, None, A, None)
+    refused(1, b"misaligned", dx, A, A, 1, 1, 8, 64, 64, A, A, A + 8, None)
+    refused(2, b"% 64", dx, A, A, 1, 1, 8, 64, 96, A, A, A, None)
+    refused(1, b"segments", dx, A, A, 0, 1, 8, 64, 64, A, A, A, None)
+    refused(1, b"unknown out_dtype", "mirai_moe_combine_f32", A, A, None, 4, 2, 64, A, 2, None)
+    refused(1, b"misaligned", "mirai_moe_combine_f32", A + 4, A, None, 4, 2, 64, A, 0, None)
+    refused(1, b"hidden", "mirai_moe_combine_f32", A, A, None, 4, 17, 64, A, 0, None)
+    back = "mirai_moe_combine_backward_rows"
+    refused(1, b"null", back, A, A, A, A, 4, 2, 64, A, None, A, None)
+    refused(1, b"misaligned", back, A + 2, A, A, A, 4, 2, 64, A, A, A, None)
+    refused(1, b"hidden", back, A, A, A, A, 4, 2, 60, A, A, A, None)
+    for name, args in ((rows, (None, None, None, 1, 1, 0, 64, 64, None, None, None, None, None, None)),
+                       (dx, (None, None, 1, 1, 0, 64, 64, None, None, None, None)),
+                       (back, (None, None, None, None, 0, 2, 64, None, None, None, None))):
+        assert getattr(lib, name)(*args) == 0  # no rows
